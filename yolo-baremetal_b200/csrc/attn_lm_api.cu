@@ -1,0 +1,131 @@
+// Host entry of the text-decoder attention (yb_lm.h): argument checks, the
+// handle with the kernels' error word, and the launch.
+#include <climits>
+#include <cmath>
+#include <string>
+
+#include "attn_lm.h"
+#include "lm.h"
+
+namespace yb {
+namespace {
+
+struct Attn {
+  int device = 0, num_sms = 148;
+  int* err = nullptr;
+};
+
+status_t bad(const char* msg) {
+  set_error(std::string("attn: ") + msg);
+  return ERROR_INVALID_DIMS;
+}
+
+bool operand_ok(const void* p, const long long* s, bool zero_batch) {
+  if (reinterpret_cast<uintptr_t>(p) % 16) return false;
+  for (int i = 0; i < 3; ++i)
+    if (s[i] < 0 || s[i] % 8 || s[i] > (1LL << 38)) return false;
+  return zero_batch || s[0] > 0;
+}
+
+// Sizes and values; pointers are checked by the run.
+status_t check_sizes(const yb_attn_args& a) {
+  if (a.B < 0 || a.Sq < 0 || a.Sk < 0 || a.Hq < 1 || a.Hkv < 1) return bad("sizes must not be negative, heads >= 1");
+  if (a.Hq % a.Hkv) return bad("Hq must be a multiple of Hkv");
+  if (a.D < 8 || a.D > kAttnMaxD || a.D % 8) return bad("D must be a multiple of 8 in [8, 128]");
+  if (a.dtype != YB_F16 && a.dtype != YB_BF16) return bad("dtype must be YB_F16 or YB_BF16");
+  if (a.Sk > (1 << 30) || a.Sq > (1 << 30) || static_cast<long long>(a.B) * a.Sq * a.Hq > INT_MAX ||
+      static_cast<long long>(a.B) * a.Hkv > (1 << 30))
+    return bad("at most 2^30 keys and 2^31 - 1 rows times heads");
+  if (!std::isfinite(a.scale) || !(a.scale > 0.f)) return bad("scale must be finite and > 0");
+  if (!std::isfinite(a.cap) || a.cap < 0.f) return bad("cap must be finite and >= 0");
+  if (a.causal != 0 && a.causal != 1) return bad("causal must be 0 or 1");
+  if (a.prefix && !a.causal) return bad("prefix needs causal");
+  return SUCCESS;
+}
+
+}  // namespace
+}  // namespace yb
+
+using namespace yb;
+
+extern "C" status_t yb_attn_create(int device, void** attn) {
+  if (!attn) return ERROR_NULL_POINTER;
+  *attn = nullptr;
+  DeviceScope scope(device);
+  if (scope.error() != cudaSuccess) return cuda_status(scope.error(), "cudaSetDevice");
+  auto* h = new (std::nothrow) Attn();
+  if (!h) return ERROR_OUT_OF_MEMORY;
+  h->device = device;
+  cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device);
+  cudaError_t e = cudaMalloc(&h->err, sizeof(int));
+  if (e == cudaSuccess) e = cudaMemset(h->err, 0, sizeof(int));
+  if (e != cudaSuccess) {
+    if (h->err) cudaFree(h->err);
+    delete h;
+    return cuda_status(e, "attn create");
+  }
+  *attn = h;
+  return SUCCESS;
+}
+
+extern "C" status_t yb_attn_workspace(void* attn, const yb_attn_args* a, size_t* bytes) {
+  if (!a || !bytes) return ERROR_NULL_POINTER;
+  *bytes = 0;
+  const status_t st = check_sizes(*a);
+  if (st != SUCCESS) return st;
+  return attn ? SUCCESS : ERROR_NULL_POINTER;
+}
+
+extern "C" status_t yb_attn_run(void* attn, const yb_attn_args* p, void* workspace, size_t workspace_bytes,
+                                void* stream) {
+  auto* h = static_cast<Attn*>(attn);
+  if (!p) return ERROR_NULL_POINTER;
+  const yb_attn_args a = *p;
+  const status_t st = check_sizes(a);
+  if (st != SUCCESS) return st;
+  if (a.B == 0 || a.Sq == 0) return h ? SUCCESS : ERROR_NULL_POINTER;
+  if (!a.q || !a.o || (a.Sk > 0 && (!a.k || !a.v))) return ERROR_NULL_POINTER;
+  if (a.o == a.q || a.o == a.k || a.o == a.v) return bad("o must not be an input");
+  // A stride of a dimension of size one is never used.
+  auto ok = [&](const void* ptr, const long long* s, int rows, int heads, bool out) {
+    const long long t[3] = {a.B > 1 ? s[0] : 8, rows > 1 ? s[1] : 8, heads > 1 ? s[2] : 8};
+    return operand_ok(ptr, t, !out) && t[1] > 0 && t[2] > 0;
+  };
+  if (!ok(a.q, a.q_stride, a.Sq, a.Hq, false) || !ok(a.o, a.o_stride, a.Sq, a.Hq, true) ||
+      (a.Sk > 0 && (!ok(a.k, a.k_stride, a.Sk, a.Hkv, false) || !ok(a.v, a.v_stride, a.Sk, a.Hkv, false))))
+    return bad("q, k, v, o: 16-byte aligned, strides multiples of 8 elements; only batch strides of inputs may be 0");
+  if (a.key_range && reinterpret_cast<uintptr_t>(a.key_range) % 8) return bad("key_range must be 8-byte aligned");
+  if (!h) return ERROR_NULL_POINTER;
+  DeviceScope scope(h->device);
+  if (scope.error() != cudaSuccess) return cuda_status(scope.error(), "cudaSetDevice");
+  (void)workspace;
+  (void)workspace_bytes;
+  return cuda_status(launch_attn_rows(a, static_cast<cudaStream_t>(stream)), "attn");
+}
+
+extern "C" status_t yb_attn_check(void* attn) {
+  auto* h = static_cast<Attn*>(attn);
+  if (!h) return ERROR_NULL_POINTER;
+  DeviceScope scope(h->device);
+  cudaError_t e = scope.error();
+  if (e == cudaSuccess) e = cudaDeviceSynchronize();
+  int k = 0;
+  if (e == cudaSuccess) e = cudaMemcpy(&k, h->err, sizeof(int), cudaMemcpyDeviceToHost);
+  if (e != cudaSuccess) return cuda_status(e, "attn check");
+  if (k) {
+    cudaMemset(h->err, 0, sizeof(int));
+    set_error("attn kernel reported error code " + std::to_string(k));
+    return ERROR_DEVICE;
+  }
+  return SUCCESS;
+}
+
+extern "C" status_t yb_attn_destroy(void* attn) {
+  if (!attn) return ERROR_NULL_POINTER;
+  const status_t st = yb_attn_check(attn);
+  auto* h = static_cast<Attn*>(attn);
+  DeviceScope scope(h->device);
+  cudaFree(h->err);
+  delete h;
+  return st;
+}

@@ -49,6 +49,8 @@ EXPORTS = {
                   "yb_cuda_weight_image", "yb_conv_debug_withhold"],
     "yb_int8.h": ["yb_int8_quantize_conv", "yb_int8_conv_create", "yb_int8_conv_ci_pad", "yb_int8_conv_run",
                   "yb_int8_conv_check", "yb_int8_conv_destroy"],
+    "yb_lm.h": ["yb_attn_create", "yb_attn_workspace", "yb_attn_run", "yb_attn_check", "yb_attn_destroy",
+                "yb_qk_norm_rope", "yb_sample"],
 }
 
 
@@ -158,6 +160,13 @@ def lib() -> C.CDLL:
         L.yb_int8_conv_run.argtypes = [C.c_void_p, C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_void_p]
         L.yb_int8_conv_check.argtypes = [C.c_void_p]
         L.yb_int8_conv_destroy.argtypes = [C.c_void_p]
+        L.yb_attn_create.argtypes = [C.c_int, C.POINTER(C.c_void_p)]
+        L.yb_attn_workspace.argtypes = [C.c_void_p, C.c_void_p, C.POINTER(C.c_size_t)]
+        L.yb_attn_run.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
+        L.yb_attn_check.argtypes = [C.c_void_p]
+        L.yb_attn_destroy.argtypes = [C.c_void_p]
+        L.yb_qk_norm_rope.argtypes = [C.c_void_p, C.c_void_p]
+        L.yb_sample.argtypes = [C.c_void_p, C.c_void_p]
         L.model_forward_profile_step_name.restype = C.c_char_p
         L.model_get_weight.restype = C.POINTER(Tensor)
         _lib = L
