@@ -76,6 +76,12 @@ status_t yb_attn_run(void* attn, const yb_attn_args* a, void* workspace, size_t 
 status_t yb_attn_check(void* attn);
 status_t yb_attn_destroy(void* attn);
 
+/* Test hook of the bounded waits, as yb_conv_debug_withhold: the next
+ * yb_attn_run issues no load and bounds its waits to 1 ms; it records the
+ * error, frees its tensor memory and ends, so that yb_attn_check reports
+ * ERROR_DEVICE and later runs are unaffected. */
+status_t yb_attn_debug_withhold(void* attn);
+
 /* --------------------------------------- norm and rotation of queries, keys
  * For each head x [D] of token t (t < length[b]) of sequence b:
  *   y_d = x_d / sqrt(mean(x^2) + eps) * (weight_d + weight_add)

@@ -290,6 +290,26 @@ def test_two_streams_and_two_captures():
     att.check()
 
 
+@pytest.mark.parametrize("Sq,Sk", [(1, 300), (2, 9000), (700, 700)])
+def test_a_wait_that_runs_out_is_reported(Sq, Sk):
+    """The next run after yb_attn_debug_withhold loads nothing: its waits give up after 1 ms, the handle reports it
+    once, and later runs are as before."""
+    import yb_ops
+    import yolo_b200 as yb
+
+    q, k, v, _ = tensors(4, Sq, Sk, 16, 8, 64, "bf16")
+    att = yb_ops.Attention(16, 8, 64, torch.bfloat16, causal=True)
+    want = att(q, k, v)
+    att.check()
+    yb.check(yb.lib().yb_attn_debug_withhold(att._h), "yb_attn_debug_withhold")
+    att(q, k, v)
+    with pytest.raises(yb.YBError):
+        att.check()
+    att.check()
+    assert torch.equal(att(q, k, v), want)
+    att.check()
+
+
 def test_refusals():
     import yb_ops
     import yolo_b200 as yb

@@ -59,6 +59,7 @@ def test_attention_needs_a_handle():
     assert L.yb_attn_workspace(None, attn_args(D=12), C.byref(n)) == yb.ERROR_INVALID_DIMS and n.value == 0
     assert L.yb_attn_check(None) == yb.ERROR_NULL_POINTER
     assert L.yb_attn_destroy(None) == yb.ERROR_NULL_POINTER
+    assert L.yb_attn_debug_withhold(None) == yb.ERROR_NULL_POINTER
     assert L.yb_attn_create(0, None) == yb.ERROR_NULL_POINTER
 
 

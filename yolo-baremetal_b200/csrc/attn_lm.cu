@@ -1,38 +1,1104 @@
-// Attention over a cache or a prompt (yb_lm.h, yb_attn_run): one warp per row.
+// Attention over a prompt or a cache (yb_lm.h, yb_attn_run) on the tensor
+// cores: S = Q K^T and O += P V as tcgen05.mma kind::f16 (fp16 or bf16
+// operands, fp32 accumulation in tensor memory), one pass over the keys with a
+// running maximum and sum.
+//
+// Rows.  A tile is 128 rows: np positions times the gp query heads that share
+// a key head, so a key block is read once for all of them, and a step of one
+// token still fills gp rows.  Every mask of the operator leaves a row one run
+// of keys [lo, hi), so a thread, which owns one row, masks with two compares,
+// and only in blocks that some row of its warp does not see whole.
+//
+// CTA (10 warps): warps 0-3 and 4-7 are two softmax pipelines, warp 8 issues
+// the UMMAs, warp 9 the TMA loads into a ring of 128-key blocks of K and V.
+// Tensor memory: S0, S1 (128 columns each; P overwrites the first half of its
+// S as packed 16-bit pairs and is read back as the A operand), O0, O1.  While
+// one pipeline does its exponentials the tensor cores work for the other.
+//   row mode    the pipelines own two row tiles and share each K and V block;
+//   split mode  the pipelines take the even and odd blocks of one row tile, and
+//               the blocks of all tiles are dealt out evenly to a grid of one
+//               CTA per SM (by the lengths on the device), so a few rows over
+//               a long cache still use the whole memory bandwidth.  A tile cut
+//               between CTAs leaves (max, sum, O) in scratch, and
+//               attn_join_kernel joins the pieces in their order.
+//
+// The running maximum is only raised when it grows by more than 2^8 (then O is
+// rescaled in place): until then weights up to 256 are as exact, and O stays
+// untouched in tensor memory.  The maximum in use never enters the result.
+//
+// A weight of zero times an infinite or NaN value would be NaN, so value rows
+// of a block that no row of the tile sees are zeroed in shared memory, and a
+// row whose O comes out non-finite under a finite sum (a value that only other
+// rows see) is computed again key by key over the keys it does see.
+//
+// Rounding: P is rounded to the operands' type (they enter the same UMMA); its
+// sum is taken before that in fp32.  O, maxima and sums are fp32 throughout.
+#include <cuda.h>
+#include <cudaTypedefs.h>
+
+#include <atomic>
 #include <cmath>
+#include <mutex>
 
 #include "attn_lm.h"
 #include "attn_row.cuh"
+#include "pdl.cuh"
+#include "sm100.cuh"
+#include "split.cuh"
 
 namespace yb {
 namespace {
 
+constexpr int kB = kAttnBlock;
+constexpr int kThreads = 320;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr uint32_t kChunkBytes = kB * 128;  // 128 rows x 64 elements, 128-byte swizzle
+constexpr uint32_t kTmemCols = 512;
+constexpr float kLog2e = 1.44269504f;
+constexpr float kRaise = 8.0f;  // log2 growth of the maximum that O is rescaled for
+constexpr int kSmemMax = 232448;
+constexpr int kCtlBytes = 3072;  // control block, after up to 1 KB of alignment
+
+template <int HDP>
+__host__ __device__ constexpr int chunks() { return HDP / 64; }
+template <int HDP, bool SPLIT>
+__host__ __device__ constexpr int q_bytes() { return (SPLIT ? 1 : 2) * chunks<HDP>() * static_cast<int>(kChunkBytes); }
+template <int HDP, bool SPLIT>
+__host__ __device__ constexpr int stages() {
+  const int n = (kSmemMax - kCtlBytes - q_bytes<HDP, SPLIT>()) / (chunks<HDP>() * static_cast<int>(kChunkBytes));
+  return n > 8 ? 8 : n;
+}
+template <int HDP, bool SPLIT>
+__host__ __device__ constexpr int smem_bytes() {
+  return q_bytes<HDP, SPLIT>() + stages<HDP, SPLIT>() * chunks<HDP>() * static_cast<int>(kChunkBytes) + kCtlBytes;
+}
+
+struct Ctl {
+  uint64_t q_full, s_full[2], p_full[2], o_full[2], o_empty, ml_full, drain;
+  uint64_t kv_full[8], kv_empty[8];
+  uint32_t tmem;
+  int abort;
+  float2 ml[kB];  // split: second pipeline's maximum and sum
+};
+static_assert(sizeof(Ctl) + 1024 <= kCtlBytes, "control block plus alignment");
+
+// ------------------------------------------------------------- PTX pieces
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  tc_mma_bf16(d, ad, bd, idesc, acc);  // kind::f16; the types are in idesc
+}
+// A from tensor memory.
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t bd, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(bd), "r"(idesc), "r"(acc)
+      : "memory");
+}
+__device__ __forceinline__ void ld32(uint32_t taddr, float* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(r[0]), "=f"(r[1]), "=f"(r[2]), "=f"(r[3]), "=f"(r[4]), "=f"(r[5]), "=f"(r[6]), "=f"(r[7]), "=f"(r[8]),
+        "=f"(r[9]), "=f"(r[10]), "=f"(r[11]), "=f"(r[12]), "=f"(r[13]), "=f"(r[14]), "=f"(r[15]), "=f"(r[16]),
+        "=f"(r[17]), "=f"(r[18]), "=f"(r[19]), "=f"(r[20]), "=f"(r[21]), "=f"(r[22]), "=f"(r[23]), "=f"(r[24]),
+        "=f"(r[25]), "=f"(r[26]), "=f"(r[27]), "=f"(r[28]), "=f"(r[29]), "=f"(r[30]), "=f"(r[31])
+      : "r"(taddr)
+      : "memory");
+}
+// Orders later uses of loaded registers behind the wait for the loads.
+__device__ __forceinline__ void ld32_dep(float* r) {
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+    asm volatile(""
+                 : "+f"(r[i]), "+f"(r[i + 1]), "+f"(r[i + 2]), "+f"(r[i + 3]), "+f"(r[i + 4]), "+f"(r[i + 5]),
+                   "+f"(r[i + 6]), "+f"(r[i + 7])
+                 :
+                 : "memory");
+}
+__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+
+// V block as the B operand [keys (K)][dims (N)]: N-major, 128-byte swizzle.
+// 64 dims are one 128-byte row of the tile; the next 64 lie a chunk further
+// (leading offset), the next 8 keys 1024 bytes further (stride offset).
+__device__ __forceinline__ uint64_t v_desc(uint32_t saddr) {
+  return static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4) | (static_cast<uint64_t>(kChunkBytes >> 4) << 16) |
+         (static_cast<uint64_t>(1024 >> 4) << 32) | (static_cast<uint64_t>(1) << 46) |
+         (static_cast<uint64_t>(2) << 61);
+}
+// fp32 accumulator, both operands bf16 or both fp16, B N-major when `bn`.
 template <typename T>
-__global__ void __launch_bounds__(128) attn_rows_kernel(const yb_attn_args a) {
-  const long long row = static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  if (row >= static_cast<long long>(a.B) * a.Sq * a.Hq) return;
-  const int h = static_cast<int>(row % a.Hq);
-  const int i = static_cast<int>(row / a.Hq % a.Sq), b = static_cast<int>(row / a.Hq / a.Sq);
-  const int q_len = clamp_len(a.q_len, b, a.Sq), k_len = clamp_len(a.k_len, b, a.Sk);
-  if (i >= q_len) return;
-  const RowSpan s = row_span(a, b, i, q_len, k_len);
-  const RowAcc r = attn_row<T>(a, b, i, h, s.pos, s.lo, s.hi);
-  const int d = 4 * (threadIdx.x & 31);
-  if (d >= a.D) return;
-  T* o = static_cast<T*>(a.o) + b * a.o_stride[0] + i * a.o_stride[1] + h * a.o_stride[2] + d;
-  for (int e = 0; e < 4; ++e) o[e] = from_f<T>(r.l == 0.f ? 0.f : r.o[e] / r.l);
+__device__ __forceinline__ uint32_t idesc_f32(int N, bool bn) {
+  constexpr uint32_t fmt = sizeof(T) == 2 && std::is_same<T, __nv_bfloat16>::value ? 1u : 0u;
+  return (1u << 4) | (fmt << 7) | (fmt << 10) | (bn ? 1u << 16 : 0u) | (static_cast<uint32_t>(N >> 3) << 17) |
+         (static_cast<uint32_t>(kB >> 4) << 24);
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// ------------------------------------------------------------ work division
+// Key blocks of tile qt of sequence b as far as the lengths tell (a document
+// range only narrows them); 0 when no row is in use, at least 1 otherwise.
+__device__ __forceinline__ int tile_blocks(const AttnPlan& p, int b, int qt) {
+  const int q_len = clamp_len(p.a.q_len, b, p.a.Sq), k_len = clamp_len(p.a.k_len, b, p.a.Sk);
+  const int i0 = qt * p.np;
+  if (i0 >= q_len) return 0;
+  int hi = k_len;
+  if (p.a.causal) {
+    hi = min(k_len, k_len - q_len + min(i0 + p.np, q_len));
+    if (p.a.prefix) hi = max(hi, min(p.a.prefix[b], k_len));
+  }
+  return max(1, (hi + kB - 1) / kB);
+}
+
+struct Piece {
+  int b = 0, hg = 0, qt = 0;
+  int off = 0, take = 0;  // key blocks [off, off + take) of `n`
+  int n = 0;
+  int slot = -1;  // scratch slot, -1: the whole tile
+};
+
+// A CTA's share of the blocks of all tiles, in the order (sequence, tile, head
+// group).  Every warp walks it by itself, lanes together.
+struct Walk {
+  long long total = 0, left = 0;
+  int bt = 0, hg = 0, off = 0, ctas = 1;
+
+  // Blocks of all (sequence, tile) pairs per lane, then the lane and pair that hold unit u.
+  __device__ void seek(const AttnPlan& p, int cta, int grid) {
+    const int lane = threadIdx.x & 31;
+    const int pairs = p.a.B * p.tiles;
+    if (p.whole) {  // tiles are dealt out whole
+      const long long segs = static_cast<long long>(pairs) * p.groups;
+      const long long s0 = segs * cta / grid, s1 = segs * (cta + 1) / grid;
+      bt = static_cast<int>(s0 / p.groups);
+      hg = static_cast<int>(s0 - static_cast<long long>(bt) * p.groups);
+      left = s1 - s0;
+      return;
+    }
+    const int per = (pairs + 31) / 32;
+    const int x0 = min(lane * per, pairs), x1 = min(x0 + per, pairs);
+    long long sum = 0;
+    for (int x = x0; x < x1; ++x) sum += tile_blocks(p, x / p.tiles, x % p.tiles);
+    sum *= p.groups;
+    long long scan = sum;
+    for (int d = 1; d < 32; d <<= 1) {
+      const long long o = __shfl_up_sync(0xFFFFFFFFu, scan, d);
+      if (lane >= d) scan += o;
+    }
+    total = __shfl_sync(0xFFFFFFFFu, scan, 31);
+    const long long want = (total + p.unit_min - 1) / p.unit_min;
+    ctas = static_cast<int>(want < 1 ? 1 : want < grid ? want : grid);
+    if (cta >= ctas) return;
+    const long long u0 = total * cta / ctas, u1 = total * (cta + 1) / ctas;
+    left = u1 - u0;
+    if (left <= 0) return;
+    const unsigned has = __ballot_sync(0xFFFFFFFFu, scan > u0);
+    const int who = __ffs(has) - 1;
+    long long rest = u0 - (scan - sum);  // of lane `who`
+    int at = x0, h = 0, o = 0;
+    if (lane == who) {
+      for (; at < x1; ++at) {
+        const long long n = static_cast<long long>(tile_blocks(p, at / p.tiles, at % p.tiles));
+        if (rest < n * p.groups) {
+          h = static_cast<int>(rest / n);
+          o = static_cast<int>(rest - h * n);
+          break;
+        }
+        rest -= n * p.groups;
+      }
+    }
+    bt = __shfl_sync(0xFFFFFFFFu, at, who);
+    hg = __shfl_sync(0xFFFFFFFFu, h, who);
+    off = __shfl_sync(0xFFFFFFFFu, o, who);
+  }
+
+  __device__ bool next(const AttnPlan& p, Piece* s) {
+    while (left > 0 && bt < p.a.B * p.tiles) {
+      s->b = bt / p.tiles;
+      s->qt = bt - s->b * p.tiles;
+      s->n = tile_blocks(p, s->b, s->qt);
+      if (s->n == 0) {
+        if (p.whole) {
+          left -= p.groups - hg;
+        }
+        ++bt;
+        hg = 0;
+        continue;
+      }
+      s->hg = hg;
+      s->off = off;
+      s->take = p.whole ? s->n : static_cast<int>(min(static_cast<long long>(s->n - off), left));
+      s->slot = s->take == s->n ? -1 : s->off ? 0 : 1;
+      left -= p.whole ? 1 : s->take;
+      off += s->take;
+      if (off >= s->n) {
+        off = 0;
+        if (++hg == p.groups) hg = 0, ++bt;
+      }
+      return true;
+    }
+    return false;
+  }
+};
+
+// Keys that some row of the tile sees: [lo, hi), by a whole warp.
+struct Keys {
+  int lo, hi;
+};
+__device__ __forceinline__ Keys tile_keys(const AttnPlan& p, int b, int qt) {
+  const int q_len = clamp_len(p.a.q_len, b, p.a.Sq), k_len = clamp_len(p.a.k_len, b, p.a.Sk);
+  const int i0 = qt * p.np, i1 = min(i0 + p.np, q_len);
+  Keys k{0, 0};
+  if (i0 >= i1) return k;
+  if (!p.a.key_range) {
+    k.hi = max(0, row_span(p.a, b, i1 - 1, q_len, k_len).hi);
+    return k;
+  }
+  int lo = 0x7FFFFFFF, hi = 0;
+  for (int i = i0 + static_cast<int>(threadIdx.x & 31); i < i1; i += 32) {
+    const RowSpan s = row_span(p.a, b, i, q_len, k_len);
+    if (s.lo < s.hi) {
+      lo = min(lo, s.lo);
+      hi = max(hi, s.hi);
+    }
+  }
+  lo = __reduce_min_sync(0xFFFFFFFFu, lo);
+  hi = __reduce_max_sync(0xFFFFFFFFu, hi);
+  if (lo < hi) k.lo = lo, k.hi = hi;
+  return k;
+}
+
+// Block range of a CTA's two pipelines.
+struct Blocks {
+  int j0[2], j1[2];  // row mode: each tile's; split mode: both hold the piece's
+  int lo, hi;        // keys outside need not be finite in V
+};
+template <bool SPLIT>
+__device__ __forceinline__ Blocks block_range(const AttnPlan& p, const Piece& s) {
+  Blocks r;
+  if constexpr (SPLIT) {
+    const Keys k = tile_keys(p, s.b, s.qt);
+    int a = k.lo / kB, e = (k.hi + kB - 1) / kB;
+    a = max(a, s.off);
+    e = max(a, min(e, s.off + s.take));
+    r.j0[0] = r.j0[1] = a;
+    r.j1[0] = r.j1[1] = e;
+    r.lo = k.lo;
+    r.hi = k.hi;
+  } else {
+    r.lo = 0x7FFFFFFF;
+    r.hi = 0;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const Keys k = tile_keys(p, s.b, s.qt + t);
+      r.j0[t] = k.lo / kB;
+      r.j1[t] = max(r.j0[t], (k.hi + kB - 1) / kB);
+      if (k.lo < k.hi) {
+        r.lo = min(r.lo, k.lo);
+        r.hi = max(r.hi, k.hi);
+      }
+    }
+    if (r.j0[0] == r.j1[0]) r.j0[0] = r.j1[0] = r.j0[1];  // an empty tile takes no part in the union
+    if (r.j0[1] == r.j1[1]) r.j0[1] = r.j1[1] = r.j0[0];
+  }
+  return r;
+}
+
+__device__ __forceinline__ void raise_error(int* err, volatile int* abort_flag, int code) {
+  *abort_flag = 1;
+  atomicCAS(err, 0, code);
+}
+
+// Position in the ring of key and value blocks.
+struct Ring {
+  int slot = 0;
+  uint32_t phase = 0;
+  template <int N>
+  __device__ __forceinline__ void next() {
+    if (++slot == N) slot = 0, phase ^= 1u;
+  }
+};
+
+// ------------------------------------------------------------------ softmax
+// One block of one row: scores in s (raw on entry), weights out as packed
+// pairs in pk, the row's maximum (log2 units) and sum updated.  Returns the
+// factor that O has to be scaled by (1: none).
+template <typename T, bool CAP, bool BIAS>
+struct RowState {
+  float m = -INFINITY, l = 0.f;
+  int lo = 0, hi = 0, pos = 0;
+  float slope = 0.f;
+  bool valid = false;
+};
+
+struct ScoreConst {
+  float sc2;       // scale * log2(e); with a cap: scale / cap
+  float cap2;      // cap * log2(e)
+  float c0, c1, c2, c3;  // cap2 * tanh(u) = u (c0 + c1 u^2 + c2 u^4 + c3 u^6) for |u| <= 1/2
+};
+
+// cap2 tanh(u) for any u: 1 - 2 / (1 + e^(2u)).
+__device__ __forceinline__ float cap_any(float u, const ScoreConst& c) {
+  return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(u * (2.0f * kLog2e))), 1.0f);
+}
+
+// cap2 tanh(sc2 s) of 32 scores in place.  Near zero (|u| <= 1/2, all 32 of
+// every row of the warp) a polynomial on the FMA pipe; its absolute error is
+// 1.5e-7 of the cap.  The exponential form takes two steps of the 16-per-clock
+// pipe that the softmax already fills.
+__device__ __forceinline__ void cap32(float* s, const ScoreConst& c) {
+  float big = 0.f;
+#pragma unroll
+  for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(s[e]), fabsf(s[e + 1])));
+  if (__all_sync(0xFFFFFFFFu, big * c.sc2 <= 0.5f)) {
+#pragma unroll
+    for (int e = 0; e < 32; e += 2) {
+      const float2 u = __fmul2_rn(make_float2(s[e], s[e + 1]), make_float2(c.sc2, c.sc2));
+      const float2 z = __fmul2_rn(u, u);
+      float2 q = __ffma2_rn(make_float2(c.c3, c.c3), z, make_float2(c.c2, c.c2));
+      q = __ffma2_rn(q, z, make_float2(c.c1, c.c1));
+      q = __ffma2_rn(q, z, make_float2(c.c0, c.c0));
+      q = __fmul2_rn(q, u);
+      s[e] = q.x;
+      s[e + 1] = q.y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 32; ++e) s[e] = cap_any(s[e] * c.sc2, c);
+  }
+}
+
+template <typename T, bool CAP, bool BIAS>
+__device__ __forceinline__ float softmax_block(float* s, uint32_t* pk, RowState<T, CAP, BIAS>& r, const ScoreConst& c,
+                                               int key0, bool masked, bool first) {
+  if constexpr (CAP) {
+#pragma unroll
+    for (int e = 0; e < kB; e += 32) cap32(s + e, c);
+  }
+  if constexpr (BIAS) {
+    const float d0 = static_cast<float>(key0 - r.pos);
+#pragma unroll
+    for (int e = 0; e < kB; ++e) {
+      const float x = CAP ? s[e] : s[e] * c.sc2;
+      s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), x);
+    }
+  }
+  if (masked) {
+    const uint32_t n = static_cast<uint32_t>(r.hi - r.lo);
+    const uint32_t k = static_cast<uint32_t>(key0 - r.lo);
+#pragma unroll
+    for (int e = 0; e < kB; ++e) s[e] = k + e < n ? s[e] : -INFINITY;
+  }
+  float mx[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mx[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+#pragma unroll
+  for (int e = 8; e < kB; e += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], fmaxf(s[e + 2 * i], s[e + 2 * i + 1]));
+  float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  constexpr bool kScaled = CAP || BIAS;  // s is in log2 units already
+  if constexpr (!kScaled) m *= c.sc2;
+  float factor = 1.0f;
+  if (first) {
+    r.m = m;
+  } else if (m > r.m + kRaise) {
+    factor = ex2_ftz(r.m - m);
+    r.l *= factor;
+    r.m = m;
+  }
+  const float base = r.m == -INFINITY ? 0.f : -r.m;
+  float2 sum[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
+  const float2 mul = make_float2(kScaled ? 1.0f : c.sc2, kScaled ? 1.0f : c.sc2), add = make_float2(base, base);
+#pragma unroll
+  for (int e = 0; e < kB; e += 2) {
+    const float2 x = make_float2(s[e], s[e + 1]);
+    const float2 y = kScaled ? __fadd2_rn(x, add) : __ffma2_rn(x, mul, add);
+    const float2 w = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
+    sum[(e >> 1) & 3] = __fadd2_rn(sum[(e >> 1) & 3], w);
+    pk[e >> 1] = pack2<T>(w.x, w.y);
+  }
+  const float2 a = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+  r.l += a.x + a.y;
+  return factor;
+}
+
+// ------------------------------------------------------------------- kernel
+template <typename T, int HDP, bool CAP, bool BIAS, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 1)
+    attn_tc_kernel(const __grid_constant__ AttnPlan p, const __grid_constant__ CUtensorMap tmq,
+                   const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv) {
+  constexpr int NCH = chunks<HDP>(), NST = stages<HDP, SPLIT>();
+  constexpr uint32_t kBlockBytes = NCH * kChunkBytes;
+  extern __shared__ uint8_t attn_lm_raw[];
+  uint8_t* base = attn_lm_raw + ((1024u - (smem_u32(attn_lm_raw) & 1023u)) & 1023u);
+  uint8_t* sq = base;
+  uint8_t* ring = base + q_bytes<HDP, SPLIT>();
+  Ctl& C = *reinterpret_cast<Ctl*>(ring + NST * kBlockBytes);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  volatile int* abort_flag = &C.abort;
+  const yb_attn_args& a = p.a;
+
+  pdl_trigger();  // the join's blocks may come up meanwhile; they wait for this grid's end
+  if (threadIdx.x == 0) {
+    mbar_init(&C.q_full, 1);
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&C.s_full[t], 1);
+      mbar_init(&C.p_full[t], 4);
+      mbar_init(&C.o_full[t], 1);
+    }
+    mbar_init(&C.o_empty, 4);
+    mbar_init(&C.ml_full, 4);
+    mbar_init(&C.drain, 1);
+    for (int i = 0; i < NST; ++i) {
+      mbar_init(&C.kv_full[i], 1);
+      mbar_init(&C.kv_empty[i], 1);
+    }
+    C.abort = 0;
+    mbar_fence_init();
+  }
+  if (warp == kMmaWarp) {
+    tmem_alloc(&C.tmem, kTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tm = C.tmem;
+  const uint32_t ts[2] = {tm, tm + kB}, to[2] = {tm + 2 * kB, tm + 2 * kB + HDP};
+
+  // Pieces of this CTA: split mode walks its share; row mode has one pair of
+  // tiles, the last rows (the most keys of a causal prompt) first.
+  Walk walk;
+  Piece pc;
+  const int ksteps = (a.D + 15) / 16;
+  const int fill = p.gp * p.np;  // rows of a full tile
+  bool more;
+  if constexpr (SPLIT) {
+    walk.seek(p, blockIdx.x, gridDim.x);
+    more = walk.next(p, &pc);
+  } else {
+    const int bh = a.B * p.groups, pairs = (p.tiles + 1) / 2;
+    const int x = blockIdx.x / bh, y = blockIdx.x - x * bh;
+    pc.b = y / p.groups;
+    pc.hg = y - pc.b * p.groups;
+    pc.qt = 2 * (pairs - 1 - x);
+    more = pc.qt * p.np < clamp_len(a.q_len, pc.b, a.Sq);
+  }
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------- loads
+    Ring rg;
+    int loads = 0;
+    while (more && !p.withhold) {
+      const Blocks r = block_range<SPLIT>(p, pc);
+      const int j0 = min(r.j0[0], r.j0[1]), j1 = max(r.j1[0], r.j1[1]);
+      const int hk = pc.hg * p.gp / (a.Hq / a.Hkv);
+      bool ok = true;
+      if (lane == 0) {
+        auto load = [&](const CUtensorMap* m, int bmul, int j) {
+          if (!mbar_wait(&C.kv_empty[rg.slot], rg.phase ^ 1u, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) raise_error(p.err, abort_flag, kErrWaitEmpty);
+            ok = false;
+            return;
+          }
+          mbar_arrive_expect_tx(&C.kv_full[rg.slot], kBlockBytes);
+          uint8_t* dst = ring + rg.slot * kBlockBytes;
+#pragma unroll
+          for (int c = 0; c < NCH; ++c)
+            tma_tile_4d(dst + c * kChunkBytes, m, 64 * c, j * kB, hk, pc.b * bmul, &C.kv_full[rg.slot]);
+          ++loads;
+          rg.next<NST>();
+        };
+        if constexpr (SPLIT) {
+          for (int j = j0; j <= j1 && ok && j1 > j0; ++j) {
+            if (j < j1) load(&tmk, p.k_bmul, j);
+            if (j > j0 && ok) load(&tmv, p.v_bmul, j - 1);
+          }
+        } else {
+          for (int j = j0; j < j1 && ok; ++j) {
+            load(&tmk, p.k_bmul, j);
+            if (ok) load(&tmv, p.v_bmul, j);
+          }
+        }
+      }
+      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+      if (!ok) break;
+      if constexpr (SPLIT)
+        more = walk.next(p, &pc);
+      else
+        more = false;
+    }
+    // After an abort, copies may still be landing in shared memory.
+    if (lane == 0 && *abort_flag) {
+      int dummy = 0;
+      const int open = loads < NST ? loads : NST;
+      for (int i = 0; i < open; ++i) {
+        rg.slot = rg.slot ? rg.slot - 1 : NST - 1;
+        if (rg.slot == NST - 1) rg.phase ^= 1u;
+        mbar_wait(&C.kv_full[rg.slot], rg.phase, &dummy, p.wait_ns);
+      }
+    }
+    __syncwarp();
+  } else if (warp == kMmaWarp) {
+    // -------------------------------------------------------------- UMMAs
+    Ring rg;
+    uint32_t p_phase[2] = {0, 0}, q_phase = 0;
+    int piece = 0;
+    bool ok = true, q_open = false;
+    const uint32_t id_s = idesc_f32<T>(kB, false), id_o = idesc_f32<T>(16 * ksteps, true);
+    const uint32_t q_tx = static_cast<uint32_t>(NCH * 128 * fill);
+    auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
+      // The lanes agree, so that none is left behind at a warp barrier.
+      if (ok && !__all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, p.wait_ns))) {
+        if (lane == 0 && !*abort_flag) raise_error(p.err, abort_flag, code);
+        ok = false;
+      }
+      return ok;
+    };
+    auto scores = [&](int t, int slot) {
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t qa = smem_u32(sq) + (SPLIT ? 0 : t) * kBlockBytes, kb = smem_u32(ring) + slot * kBlockBytes;
+        for (int k = 0; k < ksteps; ++k) {
+          const uint32_t o = (k >> 2) * kChunkBytes + (k & 3) * 32;
+          mma_ss(ts[t], sw128_kmajor_desc(qa + o), sw128_kmajor_desc(kb + o), id_s, k > 0);
+        }
+        tc_commit(&C.s_full[t]);
+      }
+      __syncwarp();
+    };
+    auto values = [&](int t, int slot, bool first, bool last) {
+      tc_fence_after();
+      if (lane == 0) {
+        const uint32_t vb = smem_u32(ring) + slot * kBlockBytes;
+#pragma unroll
+        for (int k = 0; k < kB / 16; ++k)
+          mma_ts(to[t], ts[t] + 8 * k, v_desc(vb + 2048 * k), id_o, !first || k > 0);
+        if (last) tc_commit(&C.o_full[t]);
+      }
+      __syncwarp();
+    };
+    auto release = [&](int slot) {
+      if (lane == 0) tc_commit(&C.kv_empty[slot]);
+      __syncwarp();
+    };
+    // Zeroes the value rows of block j that no row sees.
+    auto clean = [&](int slot, int j, const Blocks& r) {
+      if (j * kB >= r.lo && (j + 1) * kB <= r.hi) return;
+      uint4* v = reinterpret_cast<uint4*>(ring + slot * kBlockBytes);
+      for (int k = 0; k < kB; ++k) {
+        const int key = j * kB + k;
+        if (key >= r.lo && key < r.hi) continue;
+        if (lane < 8 * NCH)
+          v[(lane >> 3) * (kChunkBytes / 16) + k * 8 + (lane & 7)] = make_uint4(0u, 0u, 0u, 0u);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+    };
+    while (more && ok) {
+      const Blocks r = block_range<SPLIT>(p, pc);
+      const int j0 = min(r.j0[0], r.j0[1]), j1 = max(r.j1[0], r.j1[1]);
+      if (j1 > j0) {
+        // The earlier piece's scores are done (their weights were waited for).
+        if (lane == 0 && !p.withhold) {
+          mbar_arrive_expect_tx(&C.q_full, q_tx * (SPLIT ? 1 : (pc.qt + 1 < p.tiles ? 2 : 1)));
+          for (int t = 0; t < (SPLIT ? 1 : 2); ++t)
+            if (pc.qt + t < p.tiles)
+#pragma unroll
+              for (int c = 0; c < NCH; ++c)
+                tma_tile_4d(sq + t * kBlockBytes + c * kChunkBytes, &tmq, 64 * c, pc.hg * p.gp, (pc.qt + t) * p.np,
+                            pc.b * p.q_bmul, &C.q_full);
+        }
+        q_open = !p.withhold;
+        __syncwarp();
+        if (!wait(&C.q_full, q_phase, kErrWaitFull)) break;
+        q_open = false;
+        q_phase ^= 1u;
+        if constexpr (SPLIT) {
+          const int n = j1 - j0;
+          int vslot = 0;
+          uint32_t vphase = 0;
+          for (int i = 0; i < n + 2 && ok; ++i) {
+            // Ring order: K0, K1, V0, K2, V1, ...  V of block i - 2 comes
+            // after K of block i - 1.
+            if (i >= 2) {
+              const int v = i - 2, t = v & 1;
+              if (!wait(&C.kv_full[vslot], vphase, kErrWaitFull)) break;
+              clean(vslot, j0 + v, r);
+              if (v == 0 && piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
+              if (!wait(&C.p_full[t], p_phase[t], kErrWaitAccFull)) break;
+              p_phase[t] ^= 1u;
+              values(t, vslot, v < 2, v + 2 >= n);
+              release(vslot);
+            }
+            if (i < n) {
+              if (!wait(&C.kv_full[rg.slot], rg.phase, kErrWaitFull)) break;
+              scores(i & 1, rg.slot);
+              release(rg.slot);
+              rg.next<NST>();
+            }
+            if (i >= 1 && i <= n) {  // the ring's next block is V of block i - 1
+              vslot = rg.slot;
+              vphase = rg.phase;
+              rg.next<NST>();
+            }
+          }
+        } else {
+          if (!wait(&C.kv_full[rg.slot], rg.phase, kErrWaitFull)) break;
+          for (int t = 0; t < 2; ++t)
+            if (j0 >= r.j0[t] && j0 < r.j1[t]) scores(t, rg.slot);
+          release(rg.slot);
+          rg.next<NST>();
+          for (int j = j0; j < j1 && ok; ++j) {
+            const Ring v = rg;
+            rg.next<NST>();
+            const Ring k = rg;
+            const bool again = j + 1 < j1;
+            if (again) rg.next<NST>();
+            if (!wait(&C.kv_full[v.slot], v.phase, kErrWaitFull)) break;
+            clean(v.slot, j, r);
+            for (int t = 0; t < 2; ++t) {
+              if (j >= r.j0[t] && j < r.j1[t]) {
+                if (!wait(&C.p_full[t], p_phase[t], kErrWaitAccFull)) break;
+                p_phase[t] ^= 1u;
+                values(t, v.slot, j == r.j0[t], j + 1 == r.j1[t]);
+              }
+              if (again && j + 1 >= r.j0[t] && j + 1 < r.j1[t]) {
+                if (!wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
+                scores(t, k.slot);
+              }
+            }
+            if (!ok) break;
+            release(v.slot);
+            if (again) {
+              if (!wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
+              release(k.slot);
+            }
+          }
+        }
+      }
+      if (!ok) break;
+      ++piece;
+      if constexpr (SPLIT)
+        more = walk.next(p, &pc);
+      else
+        more = false;
+    }
+    // Everything issued has to finish before tensor memory goes.
+    if (lane == 0) {
+      int dummy = 0;
+      if (q_open) mbar_wait(&C.q_full, q_phase, &dummy, p.wait_ns);
+      tc_commit(&C.drain);
+      if (!mbar_wait(&C.drain, 0, &dummy, p.wait_ns)) raise_error(p.err, abort_flag, kErrDrain);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int t = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;
+    const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    const uint32_t my_s = ts[t] + lane_addr;
+    ScoreConst c;
+    if constexpr (CAP) {
+      c.sc2 = a.scale / a.cap;
+      c.cap2 = a.cap * kLog2e;
+      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 1/2.
+      c.c0 = c.cap2 * 0.99999768f;
+      c.c1 = c.cap2 * -0.33320656f;
+      c.c2 = c.cap2 * 0.13145146f;
+      c.c3 = c.cap2 * -0.043372475f;
+    } else {
+      c.sc2 = a.scale * kLog2e;
+      c.cap2 = c.c0 = c.c1 = c.c2 = c.c3 = 0.f;
+    }
+    uint32_t s_phase = 0, o_phase = 0;
+    int piece = 0;
+    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
+      // The lanes agree, so that none is left behind at a warp barrier.
+      if (ok && !__all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, p.wait_ns))) {
+        if (lane == 0 && !*abort_flag) raise_error(p.err, abort_flag, code);
+        ok = false;
+      }
+      return ok;
+    };
+    while (more && ok) {
+      const Blocks r = block_range<SPLIT>(p, pc);
+      const int qt = pc.qt + (SPLIT ? 0 : t);
+      const int i = qt * p.np + static_cast<int>(p.fd_gp.div(row)), h = pc.hg * p.gp + row - static_cast<int>(p.fd_gp.div(row)) * p.gp;
+      const int q_len = clamp_len(a.q_len, pc.b, a.Sq), k_len = clamp_len(a.k_len, pc.b, a.Sk);
+      RowState<T, CAP, BIAS> st;
+      st.valid = row < fill && i < q_len;
+      int wlo = 0, whi = 0x7FFFFFFF;
+      if (st.valid) {
+        const RowSpan sp = row_span(a, pc.b, i, q_len, k_len);
+        st.lo = wlo = sp.lo;
+        st.hi = whi = sp.hi;
+        st.pos = sp.pos;
+        if constexpr (BIAS) st.slope = a.slopes[h] * kLog2e;
+      }
+      const bool live = __any_sync(0xFFFFFFFFu, st.valid);
+      wlo = __reduce_max_sync(0xFFFFFFFFu, wlo);  // keys [wlo, whi) are seen by every row of the warp
+      whi = __reduce_min_sync(0xFFFFFFFFu, whi);
+      const int step = SPLIT ? 2 : 1;
+      const int jb = r.j0[t] + (SPLIT ? t : 0);
+      int done = 0;
+      for (int j = jb; j < r.j1[t]; j += step, ++done) {
+        if (!wait(&C.s_full[t], s_phase, kErrWaitAccFull)) break;
+        s_phase ^= 1u;
+        if (live) {
+          tc_fence_after();
+          float s[kB];
+          uint32_t pk[kB / 2];
+#pragma unroll
+          for (int e = 0; e < kB; e += 32) ld32(my_s + e, s + e);
+          tc_wait_ld();
+#pragma unroll
+          for (int e = 0; e < kB; e += 32) ld32_dep(s + e);
+          const bool masked = j * kB < wlo || (j + 1) * kB > whi;
+          const float f = softmax_block<T, CAP, BIAS>(s, pk, st, c, j * kB, masked, done == 0);
+          st32(my_s, pk);
+          st32(my_s + 32, pk + 32);
+          if (__any_sync(0xFFFFFFFFu, f != 1.0f)) {
+            // The product of the block before is complete: these scores were
+            // issued after it.
+            for (int e = 0; e < 16 * ksteps; e += 16) {
+              uint32_t o[16];
+              tc_ld_32x32b_x16(to[t] + lane_addr + e, o);
+              tc_wait_ld();
+              tc_ld_dep(o);
+#pragma unroll
+              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+              tc_st_32x32b_x16(to[t] + lane_addr + e, o);
+            }
+          }
+          tc_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&C.p_full[t]);
+      }
+      if (!ok) break;
+      if (done) {
+        if (!wait(&C.o_full[t], o_phase, kErrWaitAccFull)) break;
+        o_phase ^= 1u;
+      }
+      float w[2] = {1.f, 0.f}, m = st.m, l = st.l;
+      bool have[2] = {done > 0, false};
+      if constexpr (SPLIT) {
+        if (t == 1) {
+          if (piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
+          C.ml[row] = make_float2(st.m, st.l);
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&C.ml_full);
+          ++piece;
+          more = walk.next(p, &pc);
+          continue;
+        }
+        if (!wait(&C.ml_full, piece & 1, kErrWaitAccFull)) break;
+        const float2 o = C.ml[row];
+        have[1] = r.j1[0] - r.j0[0] > 1;
+        m = fmaxf(st.m, o.x);
+        const float mb = m == -INFINITY ? 0.f : m;
+        w[0] = ex2_ftz(st.m - mb);
+        w[1] = ex2_ftz(o.x - mb);
+        l = st.l * w[0] + o.y * w[1];
+      }
+      tc_fence_after();
+      const bool part = SPLIT && pc.slot >= 0;
+      const float inv = part ? 1.0f : (l == 0.f ? 0.f : 1.0f / l);
+      w[0] *= inv;
+      w[1] *= inv;
+      float* po = nullptr;
+      if (SPLIT && part) {
+        po = p.ws + (static_cast<size_t>(blockIdx.x) * 2 + pc.slot) * p.rows * (a.D + 4);
+      }
+      T* out = static_cast<T*>(a.o) + pc.b * a.o_stride[0] + static_cast<long long>(i) * a.o_stride[1] +
+               static_cast<long long>(h) * a.o_stride[2];
+      bool bad = false;
+      if (live) {
+        for (int e = 0; e < 16 * ksteps; e += 16) {
+          uint32_t x[2][16];
+#pragma unroll
+          for (int u = 0; u < (SPLIT ? 2 : 1); ++u)
+            if (have[u]) tc_ld_32x32b_x16(to[SPLIT ? u : t] + lane_addr + e, x[u]);
+          tc_wait_ld();
+          float y[16];
+#pragma unroll
+          for (int d = 0; d < 16; ++d) y[d] = 0.f;
+#pragma unroll
+          for (int u = 0; u < (SPLIT ? 2 : 1); ++u)
+            if (have[u]) {
+              tc_ld_dep(x[u]);
+#pragma unroll
+              for (int d = 0; d < 16; ++d) y[d] = fmaf(__uint_as_float(x[u][d]), w[u], y[d]);
+            }
+#pragma unroll
+          for (int d = 0; d < 16; ++d) bad = bad || !(fabsf(y[d]) <= 3.4028234e38f);
+          if (!st.valid) continue;
+          if (part) {
+            float4* dst = reinterpret_cast<float4*>(po + static_cast<size_t>(row) * a.D + e);
+#pragma unroll
+            for (int d = 0; d < 16; d += 4)
+              if (e + d < a.D) dst[d / 4] = make_float4(y[d], y[d + 1], y[d + 2], y[d + 3]);
+          } else {
+            uint32_t z[8];
+#pragma unroll
+            for (int d = 0; d < 8; ++d) z[d] = pack2<T>(y[2 * d], y[2 * d + 1]);
+            *reinterpret_cast<uint4*>(out + e) = make_uint4(z[0], z[1], z[2], z[3]);
+            if (e + 8 < a.D) *reinterpret_cast<uint4*>(out + e + 8) = make_uint4(z[4], z[5], z[6], z[7]);
+          }
+        }
+        if (part && st.valid)
+          *reinterpret_cast<float2*>(po + static_cast<size_t>(p.rows) * a.D + 2 * row) = make_float2(m, l);
+        // Rows that a value of keys they do not see has spoilt.
+        unsigned again = __ballot_sync(0xFFFFFFFFu, st.valid && bad && l == l);
+        while (again) {
+          const int who = __ffs(again) - 1;
+          again &= again - 1;
+          const int wi = __shfl_sync(0xFFFFFFFFu, i, who), wh = __shfl_sync(0xFFFFFFFFu, h, who);
+          const int pos = __shfl_sync(0xFFFFFFFFu, st.pos, who);
+          int lo = __shfl_sync(0xFFFFFFFFu, st.lo, who), hi = __shfl_sync(0xFFFFFFFFu, st.hi, who);
+          if constexpr (SPLIT) {
+            lo = max(lo, r.j0[0] * kB);
+            hi = min(hi, r.j1[0] * kB);
+          }
+          const RowAcc x = attn_row<T>(a, pc.b, wi, wh, pos, lo, hi);
+          const int d = 4 * lane, wrow = __shfl_sync(0xFFFFFFFFu, row, who);
+          if (d < a.D) {
+            if (part) {
+              *reinterpret_cast<float4*>(po + static_cast<size_t>(wrow) * a.D + d) =
+                  make_float4(x.o[0], x.o[1], x.o[2], x.o[3]);
+              if (lane == 0)
+                *reinterpret_cast<float2*>(po + static_cast<size_t>(p.rows) * a.D + 2 * wrow) = make_float2(x.m, x.l);
+            } else {
+              T* o = static_cast<T*>(a.o) + pc.b * a.o_stride[0] + static_cast<long long>(wi) * a.o_stride[1] +
+                     static_cast<long long>(wh) * a.o_stride[2] + d;
+              for (int e = 0; e < 4; ++e) o[e] = from_f<T>(x.l == 0.f ? 0.f : x.o[e] / x.l);
+            }
+          }
+        }
+      }
+      ++piece;
+      if constexpr (SPLIT) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&C.o_empty);
+        more = walk.next(p, &pc);
+      } else {
+        more = false;
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tm, kTmemCols);
+  }
+}
+
+// Joins the pieces of a tile that was cut between CTAs of the split mode.
+// Block c finds the tile, if any, whose last piece is CTA c's first and which
+// began before; its pieces lie in CTAs c0 .. c (a CTA's piece that begins the
+// tile in slot 1, later ones in slot 0).  One warp per row, pieces in order.
+template <typename T>
+__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnPlan p) {
+  const yb_attn_args& a = p.a;
+  const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Walk w;
+  w.seek(p, c, gridDim.x);
+  Piece s;
+  const bool mine = w.next(p, &s) && s.slot == 0 && s.off + s.take == s.n;
+  pdl_wait();
+  if (!mine) return;
+  const long long u0 = w.total * c / w.ctas - s.off;  // the tile's first unit
+  int c0 = c;
+  while (c0 > 0 && w.total * c0 / w.ctas > u0) --c0;
+  const int q_len = clamp_len(a.q_len, s.b, a.Sq);
+  const size_t slot_size = static_cast<size_t>(p.rows) * (a.D + 4);
+  for (int row = warp; row < p.rows; row += 8) {
+    const int x = static_cast<int>(p.fd_gp.div(row)), i = s.qt * p.np + x, h = s.hg * p.gp + row - x * p.gp;
+    if (i >= q_len) break;
+    float m = -INFINITY;
+    for (int k = c0; k <= c; ++k) {
+      const float* ml = p.ws + (2 * static_cast<size_t>(k) + (k == c0)) * slot_size + static_cast<size_t>(p.rows) * a.D;
+      m = fmaxf(m, ml[2 * row]);
+    }
+    const float mb = m == -INFINITY ? 0.f : m;
+    float l = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    const int d = 4 * lane;
+    for (int k = c0; k <= c; ++k) {
+      const float* sl = p.ws + (2 * static_cast<size_t>(k) + (k == c0)) * slot_size;
+      const float2 ml = *reinterpret_cast<const float2*>(sl + static_cast<size_t>(p.rows) * a.D + 2 * row);
+      const float f = ex2_ftz(ml.x - mb);
+      l = fmaf(ml.y, f, l);
+      if (d < a.D) {
+        const float4 v = *reinterpret_cast<const float4*>(sl + static_cast<size_t>(row) * a.D + d);
+        o.x = fmaf(v.x, f, o.x);
+        o.y = fmaf(v.y, f, o.y);
+        o.z = fmaf(v.z, f, o.z);
+        o.w = fmaf(v.w, f, o.w);
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.0f / l;
+    if (d < a.D)
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + s.b * a.o_stride[0] + static_cast<long long>(i) * a.o_stride[1] +
+                                static_cast<long long>(h) * a.o_stride[2] + d) =
+          make_uint2(pack2<T>(o.x * inv, o.y * inv), pack2<T>(o.z * inv, o.w * inv));
+  }
+}
+
+// --------------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 tiled_encoder() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  });
+  return fn;
+}
+
+// Map over [B, rows, heads, D] with boxes of 64 dims.  order_rows: box rows run
+// over positions (K, V; dims D, row, head, batch), else over heads, then
+// positions (Q; dims D, head, row, batch).
+bool encode(CUtensorMap* map, const yb_attn_args& a, const void* base, const long long* st, int rows, int heads,
+            bool order_rows, int box1, int box2, bool one_batch) {
+  const auto enc = tiled_encoder();
+  if (!enc) return false;
+  auto bytes = [](long long s, int n) { return static_cast<cuuint64_t>(n > 1 ? s * 2 : 16); };
+  const cuuint64_t nr = rows > 0 ? rows : 1, nh = heads, nb = one_batch ? 1 : a.B;
+  const cuuint64_t sr = bytes(st[1], rows), sh = bytes(st[2], heads), sb = bytes(st[0], static_cast<int>(nb));
+  cuuint64_t dims[4] = {static_cast<cuuint64_t>(a.D), order_rows ? nr : nh, order_rows ? nh : nr, nb};
+  cuuint64_t strides[3] = {order_rows ? sr : sh, order_rows ? sh : sr, sb};
+  cuuint32_t box[4] = {64, static_cast<cuuint32_t>(box1), static_cast<cuuint32_t>(box2), 1};
+  cuuint32_t estr[4] = {1, 1, 1, 1};
+  return enc(map, a.dtype == YB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
+             const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+             CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// Calls f with the kernel for these options.
+template <typename T, int HDP, bool CAP, bool BIAS, typename F>
+cudaError_t pick_mode(bool split, F f) {
+  if (split) return f(attn_tc_kernel<T, HDP, CAP, BIAS, true>, smem_bytes<HDP, true>());
+  return f(attn_tc_kernel<T, HDP, CAP, BIAS, false>, smem_bytes<HDP, false>());
+}
+template <typename T, int HDP, typename F>
+cudaError_t pick_score(bool cap, bool bias, bool split, F f) {
+  if (cap && bias) return pick_mode<T, HDP, true, true>(split, f);
+  if (cap) return pick_mode<T, HDP, true, false>(split, f);
+  if (bias) return pick_mode<T, HDP, false, true>(split, f);
+  return pick_mode<T, HDP, false, false>(split, f);
+}
+template <typename F>
+cudaError_t pick(int dtype, int hdp, bool cap, bool bias, bool split, F f) {
+  if (dtype == YB_F16)
+    return hdp == 64 ? pick_score<__half, 64>(cap, bias, split, f) : pick_score<__half, 128>(cap, bias, split, f);
+  return hdp == 64 ? pick_score<__nv_bfloat16, 64>(cap, bias, split, f)
+                   : pick_score<__nv_bfloat16, 128>(cap, bias, split, f);
 }
 
 }  // namespace
 
-cudaError_t launch_attn_rows(const yb_attn_args& a, cudaStream_t s) {
-  const long long rows = static_cast<long long>(a.B) * a.Sq * a.Hq;
-  const unsigned grid = static_cast<unsigned>((rows + 3) / 4);
-  if (a.dtype == YB_F16)
-    attn_rows_kernel<__half><<<grid, 128, 0, s>>>(a);
-  else
-    attn_rows_kernel<__nv_bfloat16><<<grid, 128, 0, s>>>(a);
-  return cudaGetLastError();
+AttnPlan plan_attn(const yb_attn_args& a, int num_sms) {
+  AttnPlan p;
+  p.a = a;
+  const int share = a.Hq / a.Hkv;
+  p.gp = share <= kB ? share : 1;
+  p.np = kB / p.gp;
+  p.groups = a.Hq / p.gp;
+  p.tiles = (a.Sq + p.np - 1) / p.np;
+  p.rows = p.gp * (p.np < a.Sq ? p.np : a.Sq);
+  p.q_bmul = a.B > 1 && a.q_stride[0] == 0 ? 0 : 1;
+  p.k_bmul = a.B > 1 && a.k_stride[0] == 0 ? 0 : 1;
+  p.v_bmul = a.B > 1 && a.v_stride[0] == 0 ? 0 : 1;
+  p.fd_gp = FastDiv(static_cast<uint32_t>(p.gp));
+  const long long segs = static_cast<long long>(a.B) * p.tiles * p.groups;
+  const int blocks = (a.Sk + kB - 1) / kB;
+  p.split = p.tiles == 1 || segs <= num_sms;
+  if (p.split) {
+    p.whole = blocks <= 4;
+    p.unit_min = 4;
+    const long long most = p.whole ? segs : segs * blocks;
+    p.grid = static_cast<int>(most < num_sms ? most : num_sms);
+  } else {
+    p.grid = static_cast<int>(static_cast<long long>(a.B) * p.groups * ((p.tiles + 1) / 2));
+  }
+  return p;
+}
+
+size_t attn_workspace_bytes(const AttnPlan& p) {
+  if (!p.split || p.whole) return 0;
+  return static_cast<size_t>(p.grid) * 2 * p.rows * (p.a.D + 4) * sizeof(float);
+}
+
+cudaError_t prepare_attn() {
+  for (int dt : {YB_F16, YB_BF16})
+    for (int hdp : {64, 128})
+      for (int o = 0; o < 8; ++o) {
+        const cudaError_t e = pick(dt, hdp, o & 1, o & 2, o & 4, [](auto kernel, int smem) {
+          return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        });
+        if (e != cudaSuccess) return e;
+      }
+  cudaFuncAttributes fa;
+  cudaError_t e = cudaFuncGetAttributes(&fa, attn_join_kernel<__half>);
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, attn_join_kernel<__nv_bfloat16>);
+  return e;
+}
+
+cudaError_t launch_attn(const AttnPlan& p, cudaStream_t s) {
+  const yb_attn_args& a = p.a;
+  CUtensorMap tmq, tmk, tmv;
+  const void* k = a.Sk ? a.k : a.q;
+  const void* v = a.Sk ? a.v : a.q;
+  if (!encode(&tmq, a, a.q, a.q_stride, a.Sq, a.Hq, false, p.gp, p.np, !p.q_bmul) ||
+      !encode(&tmk, a, k, a.k_stride, a.Sk, a.Hkv, true, kB, 1, !p.k_bmul) ||
+      !encode(&tmv, a, v, a.v_stride, a.Sk, a.Hkv, true, kB, 1, !p.v_bmul))
+    return cudaErrorInvalidValue;
+  cudaError_t e = pick(a.dtype, a.D <= 64 ? 64 : 128, a.cap > 0.f, a.slopes != nullptr, p.split,
+                       [&](auto kernel, int smem) {
+                         kernel<<<p.grid, kThreads, smem, s>>>(p, tmq, tmk, tmv);
+                         return cudaGetLastError();
+                       });
+  if (e != cudaSuccess || !p.split || p.whole) return e;
+  const dim3 grid(static_cast<unsigned>(p.grid));
+  if (a.dtype == YB_F16) return launch_pdl(attn_join_kernel<__half>, grid, dim3(256), 0, s, p);
+  return launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, p);
 }
 
 }  // namespace yb

@@ -1,11 +1,14 @@
 // Host entry of the text-decoder attention (yb_lm.h): argument checks, the
 // handle with the kernels' error word, and the launch.
+#include <atomic>
 #include <climits>
 #include <cmath>
+#include <new>
 #include <string>
 
 #include "attn_lm.h"
 #include "lm.h"
+#include "sm100.cuh"
 
 namespace yb {
 namespace {
@@ -13,6 +16,7 @@ namespace {
 struct Attn {
   int device = 0, num_sms = 148;
   int* err = nullptr;
+  std::atomic<bool> withhold_next{false};  // test hook armed by yb_attn_debug_withhold
 };
 
 status_t bad(const char* msg) {
@@ -57,7 +61,8 @@ extern "C" status_t yb_attn_create(int device, void** attn) {
   if (!h) return ERROR_OUT_OF_MEMORY;
   h->device = device;
   cudaDeviceGetAttribute(&h->num_sms, cudaDevAttrMultiProcessorCount, device);
-  cudaError_t e = cudaMalloc(&h->err, sizeof(int));
+  cudaError_t e = prepare_attn();
+  if (e == cudaSuccess) e = cudaMalloc(&h->err, sizeof(int));
   if (e == cudaSuccess) e = cudaMemset(h->err, 0, sizeof(int));
   if (e != cudaSuccess) {
     if (h->err) cudaFree(h->err);
@@ -73,7 +78,9 @@ extern "C" status_t yb_attn_workspace(void* attn, const yb_attn_args* a, size_t*
   *bytes = 0;
   const status_t st = check_sizes(*a);
   if (st != SUCCESS) return st;
-  return attn ? SUCCESS : ERROR_NULL_POINTER;
+  if (!attn) return ERROR_NULL_POINTER;
+  if (a->B && a->Sq) *bytes = attn_workspace_bytes(plan_attn(*a, static_cast<Attn*>(attn)->num_sms));
+  return SUCCESS;
 }
 
 extern "C" status_t yb_attn_run(void* attn, const yb_attn_args* p, void* workspace, size_t workspace_bytes,
@@ -98,9 +105,24 @@ extern "C" status_t yb_attn_run(void* attn, const yb_attn_args* p, void* workspa
   if (!h) return ERROR_NULL_POINTER;
   DeviceScope scope(h->device);
   if (scope.error() != cudaSuccess) return cuda_status(scope.error(), "cudaSetDevice");
-  (void)workspace;
-  (void)workspace_bytes;
-  return cuda_status(launch_attn_rows(a, static_cast<cudaStream_t>(stream)), "attn");
+  AttnPlan plan = plan_attn(a, h->num_sms);
+  const size_t need = attn_workspace_bytes(plan);
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16))
+    return bad("workspace must be 16-byte aligned and hold yb_attn_workspace bytes");
+  plan.ws = static_cast<float*>(workspace);
+  plan.err = h->err;
+  plan.wait_ns = kWaitNs;
+  if (h->withhold_next.exchange(false)) {
+    plan.withhold = 1;
+    plan.wait_ns = 1000000;  // 1 ms
+  }
+  return cuda_status(launch_attn(plan, static_cast<cudaStream_t>(stream)), "attn");
+}
+
+extern "C" status_t yb_attn_debug_withhold(void* attn) {
+  if (!attn) return ERROR_NULL_POINTER;
+  static_cast<Attn*>(attn)->withhold_next = true;
+  return SUCCESS;
 }
 
 extern "C" status_t yb_attn_check(void* attn) {

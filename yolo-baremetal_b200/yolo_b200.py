@@ -50,7 +50,7 @@ EXPORTS = {
     "yb_int8.h": ["yb_int8_quantize_conv", "yb_int8_conv_create", "yb_int8_conv_ci_pad", "yb_int8_conv_run",
                   "yb_int8_conv_check", "yb_int8_conv_destroy"],
     "yb_lm.h": ["yb_attn_create", "yb_attn_workspace", "yb_attn_run", "yb_attn_check", "yb_attn_destroy",
-                "yb_qk_norm_rope", "yb_sample"],
+                "yb_attn_debug_withhold", "yb_qk_norm_rope", "yb_sample"],
 }
 
 
@@ -165,6 +165,7 @@ def lib() -> C.CDLL:
         L.yb_attn_run.argtypes = [C.c_void_p, C.c_void_p, C.c_void_p, C.c_size_t, C.c_void_p]
         L.yb_attn_check.argtypes = [C.c_void_p]
         L.yb_attn_destroy.argtypes = [C.c_void_p]
+        L.yb_attn_debug_withhold.argtypes = [C.c_void_p]
         L.yb_qk_norm_rope.argtypes = [C.c_void_p, C.c_void_p]
         L.yb_sample.argtypes = [C.c_void_p, C.c_void_p]
         L.model_forward_profile_step_name.restype = C.c_char_p
