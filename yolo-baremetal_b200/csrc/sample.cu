@@ -9,15 +9,19 @@
 // 100,000 tokens is a whole token).
 //
 // One cluster of C CTAs per row; each keeps its slice of the row in shared
-// memory as order-preserving 32-bit keys, so the logits are read once.
-//   1 keys, and the row's largest (key, lowest index);
-//   2 with top-k or top-p: a histogram of counts and weights over 1/16-octave
-//     steps below the maximum, summed over the cluster; the step that holds
-//     the border is either listed (at most kList tokens, ranked by comparing
-//     all pairs) or split again into kBins by its composites (key, ~index),
-//     which are all distinct, so ties need no rule of their own;
-//   3 sums of the kept weights per warp and CTA, then the one warp that holds
-//     the border walks its tokens.
+// memory, so the logits are read once.
+//   1 the row's largest (logit, lowest index);
+//   2 with top-k or top-p: a histogram over 1/16-octave steps of the weight
+//     below the maximum, summed over the cluster: counts alone (fp32) for
+//     top-k, weights as well for top-p; it names the step that holds the
+//     border;
+//   3a at most kList tokens down to that step (the usual case): all go to CTA 0,
+//     which ranks them by comparing all pairs and finishes the row;
+//   3b else the step that holds the border is split further by composites
+//     (order-preserving key, ~index), which are all distinct, so ties need no
+//     rule of their own, until kList of them are left to rank; what stays
+//     above the cut is summed per warp and CTA, and the 32 runs of the CTA that
+//     holds the goal are scanned.
 #include <cooperative_groups.h>
 
 #include <atomic>
@@ -36,37 +40,53 @@ namespace {
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kBins = 1024;
+constexpr int kLive = 46 * 16;  // steps from here on weigh less than 2^-45: never chosen
 constexpr int kList = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSlice = YB_SAMPLE_MAX_VOCAB / kMaxCluster;
+constexpr int kCopies = 16;  // of the table, so that a warp's look-ups never share a bank
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 using u64 = unsigned long long;
 
-struct SampleSmem {
-  u64 tmass[kBins];   // cluster totals
+struct alignas(16) SampleSmem {
+  double table[64 * kCopies];  // 2^(j / 64)
+  u64 warp_a[kWarps], warp_b[kWarps];
+  u64 slot_a[kMaxCluster], slot_b[kMaxCluster], slot_best[kMaxCluster], slot_sum[kMaxCluster];
+};
+struct alignas(16) FilterSmem {
+  u64 tmass[kBins];  // cluster totals
   uint32_t tcnt[kBins];
   uint32_t cnt[kBins];      // own slice; the weights' sums in three 15-bit parts
   uint32_t part[3][kBins];  // (2^15 tokens of a slice: 30 bits each)
   u64 list[kList];
   u64 list_w[kList];
-  double table[64];  // 2^(j / 64)
-  u64 warp_a[kWarps], warp_b[kWarps];
-  u64 slot_a[kMaxCluster], slot_b[kMaxCluster];
   u64 result[2];
-  int found[1];
+  int found;
   int n_list;
 };
 
-__device__ __forceinline__ uint32_t key_of(float x) {
-  // NaN and -infinity: 0, which no kept logit has.
-  if (!(x >= -FLT_MAX)) return 0u;
-  x = fminf(x, FLT_MAX) + 0.0f;  // -0 and 0 are equal
-  const uint32_t b = __float_as_uint(x);
-  return b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+// NaN, -infinity: -infinity, which is never chosen; +infinity: the largest float.
+__device__ __forceinline__ float clean(float x) {
+  return x >= -FLT_MAX ? fminf(x, FLT_MAX) + 0.0f : -INFINITY;  // -0 and 0 are equal
 }
-__device__ __forceinline__ float val_of(uint32_t k) {
+__device__ __forceinline__ u64 composite(float x, uint32_t idx) {
+  const uint32_t b = __float_as_uint(x);
+  const uint32_t k = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
+  return (static_cast<u64>(x == -INFINITY ? 0u : k) << 32) | (0xFFFFFFFFu - idx);
+}
+__device__ __forceinline__ float value_of(u64 c) {
+  const uint32_t k = static_cast<uint32_t>(c >> 32);
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
+}
+
+// fp32 -> fp64 on the integer pipe (the conversion instruction runs at a
+// quarter of the fp64 rate); subnormals become zero.
+__device__ __forceinline__ double widen(float x) {
+  const uint32_t b = __float_as_uint(x);
+  const bool tiny = (b & 0x7F800000u) == 0u;
+  const uint32_t hi = (b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + (896u << 20));
+  return __hiloint2double(tiny ? 0 : static_cast<int>(hi), tiny ? 0 : static_cast<int>(b << 29));
 }
 
 struct Row {
@@ -74,34 +94,29 @@ struct Row {
   float bestf = 0, cf = 0;
 };
 
-// rint(2^44 2^y), y = (x - best) log2(e) / T <= 0.  2^y = 2^n 2^(j/64) e^r with
-// |r| <= ln 2 / 128 (table-driven, after Tang 1989): the Taylor polynomial of
-// degree 6 leaves r^7 / 5040 < 2^-64.
-__device__ __forceinline__ u64 weight(uint32_t key, const Row& r, const double* table) {
-  if (key == 0u) return 0ull;
-  const double y = (static_cast<double>(val_of(key)) - r.best) * r.c;
-  if (!(y > -46.0)) return 0ull;
-  const double t = rint(y * 64.0);
-  const int k = static_cast<int>(t);
-  const double q = (y - t * 0.015625) * 0.69314718055994530942;
-  double p = fma(q, 1.0 / 720.0, 1.0 / 120.0);
-  p = fma(p, q, 1.0 / 24.0);
-  p = fma(p, q, 1.0 / 6.0);
-  p = fma(p, q, 0.5);
+// rint(2^44 2^y), y = (x - best) log2(e) / T <= 0.  2^y = 2^n 2^(j/64) 2^r with
+// |r| <= 1/128 (table-driven, after Tang 1989): the Taylor polynomial of degree
+// 4 leaves (r ln 2)^5 / 120 < 2^-44.  Ten fp64 operations, no conversion:
+// rounding to whole numbers is done by adding 1.5 2^52 and 2^52.
+__device__ __forceinline__ u64 weight(float x, const Row& r, const double* table) {
+  const double y = (widen(x) - r.best) * r.c;
+  const double t = fma(y, 64.0, 6755399441055744.0);
+  const int k = __double2loint(t);
+  const double q = fma(t - 6755399441055744.0, -0.015625, y);
+  double p = fma(q, 9.6181291076284771619e-3, 5.5504108664821579953e-2);  // ln2^4 / 24, ln2^3 / 6
+  p = fma(p, q, 0.24022650695910071233);                                  // ln2^2 / 2
+  p = fma(p, q, 0.69314718055994530942);
   p = fma(p, q, 1.0);
-  p = fma(p, q, 1.0);
-  const double s = __longlong_as_double(static_cast<long long>(1023 + 44 + (k >> 6)) << 52);
-  return static_cast<u64>(__double2ull_rn(p * table[k & 63] * s));
+  p *= table[(k & 63) * kCopies + (threadIdx.x & (kCopies - 1))];
+  const double v = __hiloint2double(__double2hiint(p) + (((k >> 6) + 44) << 20), __double2loint(p)) + 4503599627370496.0;
+  const u64 w = static_cast<u64>(__double_as_longlong(v)) & 0xFFFFFFFFFFFFFull;
+  return y > -46.0 && x > -INFINITY ? w : 0ull;
 }
 
-// Step of 1/16 octave below the maximum: rises as the key falls.
-__device__ __forceinline__ int step_of(uint32_t key, const Row& r) {
-  const float d = (r.bestf - val_of(key)) * r.cf * 16.0f;
-  return d < static_cast<float>(kBins - 1) ? static_cast<int>(d) : kBins - 1;
-}
-
-__device__ __forceinline__ u64 composite(uint32_t key, uint32_t idx) {
-  return (static_cast<u64>(key) << 32) | (0xFFFFFFFFu - idx);
+// Step of 1/16 octave below the maximum: rises as the logit falls.
+__device__ __forceinline__ int step_of(float x, const Row& r) {
+  const float d = (r.bestf - x) * r.cf;
+  return d < static_cast<float>(kLive) ? static_cast<int>(d) : kLive;
 }
 
 __device__ __forceinline__ u64 shfl_xor64(u64 v, int m) { return __shfl_xor_sync(0xFFFFFFFFu, v, m); }
@@ -127,13 +142,13 @@ struct AddOp {
   __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
 };
 
-// The same value in every thread of the cluster.  Each use of a slot array is
-// separated from the next by the cluster barrier of the other kind of use.
+// The same value in every thread of the cluster.  The slots' earlier readers
+// are done once the caller is behind a cluster barrier of its own (`sync`).
 template <typename Op>
-__device__ u64 cluster_reduce(cg::cluster_group& cl, u64 v, SampleSmem& S, u64* slot, u64 id, Op op) {
+__device__ u64 cluster_reduce(cg::cluster_group& cl, u64 v, SampleSmem& S, u64* slot, u64 id, Op op, bool sync) {
   const u64 b = block_reduce(v, S.warp_a, id, op);
   const unsigned C = cl.num_blocks(), me = cl.block_rank();
-  cl.sync();  // earlier readers of the slots are done
+  if (sync) cl.sync();
   if (threadIdx.x < C) cl.map_shared_rank(slot, threadIdx.x)[me] = b;
   cl.sync();
   u64 r = id;
@@ -141,33 +156,61 @@ __device__ u64 cluster_reduce(cg::cluster_group& cl, u64 v, SampleSmem& S, u64* 
   return r;
 }
 
+struct Settings {
+  int top_k = 0;
+  float top_p = 1.0f, u = 0.f;
+  u64 least = 0;  // min-p as a weight
+};
+
+__device__ __forceinline__ u64 mass_target(float top_p, u64 mass) {
+  // A token is kept while the weight before it is below top_p times the whole.
+  return static_cast<u64>(fmax(1.0, ceil(static_cast<double>(top_p) * static_cast<double>(mass))));
+}
+__device__ __forceinline__ u64 goal_of(float u, u64 all) {
+  const u64 g = static_cast<u64>(fmin(static_cast<double>(u), 1.0) * static_cast<double>(all));
+  return g < all ? g : all - 1;
+}
+__device__ __forceinline__ void answer(const yb_sample_args& a, int b, uint32_t token, u64 w, u64 all) {
+  a.token[b] = static_cast<int>(token);
+  if (a.logprob) a.logprob[b] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
+}
+
 struct Picker {
   cg::cluster_group& cl;
   SampleSmem& S;
-  const uint32_t* keys;
+  FilterSmem& F;
+  const float* x;
   int n;          // tokens of the slice
   uint32_t base;  // index of its first
   Row row;
 
-  // Adds one token to bin b of the own histogram.
-  __device__ void add(int b, u64 w, bool with_mass) {
-    atomicAdd(&S.cnt[b], 1u);
-    if (with_mass) {
-      const uint32_t p0 = w & 0x7FFFu, p1 = (w >> 15) & 0x7FFFu, p2 = static_cast<uint32_t>(w >> 30);
-      if (p0) atomicAdd(&S.part[0][b], p0);
-      if (p1) atomicAdd(&S.part[1][b], p1);
-      if (p2) atomicAdd(&S.part[2][b], p2);
-    }
-  }
-  __device__ void clear() {
+  __device__ void clear(bool with_mass) {
     for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      S.cnt[b] = 0;
-      S.part[0][b] = S.part[1][b] = S.part[2][b] = 0;
+      F.cnt[b] = 0;
+      if (with_mass) F.part[0][b] = F.part[1][b] = F.part[2][b] = 0;
     }
     __syncthreads();
   }
-  // Cluster totals of the histogram into tcnt, tmass of every CTA: CTA r sums
-  // the bins congruent to its share and writes them to all.
+  // Adds one token to bin b of the own histogram.
+  __device__ void add(int b, u64 w, bool with_mass) {
+    atomicAdd(&F.cnt[b], 1u);
+    if (with_mass) {
+      const uint32_t p0 = w & 0x7FFFu, p1 = (w >> 15) & 0x7FFFu, p2 = static_cast<uint32_t>(w >> 30);
+      if (p0) atomicAdd(&F.part[0][b], p0);
+      if (p1) atomicAdd(&F.part[1][b], p1);
+      if (p2) atomicAdd(&F.part[2][b], p2);
+    }
+  }
+  __device__ void steps(bool with_mass) {
+    clear(with_mass);
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int b = step_of(x[i], row);
+      if (b < kLive) add(b, with_mass ? weight(x[i], row, S.table) : 0ull, with_mass);
+    }
+    total(with_mass);
+  }
+  // Cluster totals of the histogram into tcnt, tmass of every CTA: each CTA
+  // sums its share of the bins and writes them to all.
   __device__ void total(bool with_mass) {
     const int C = static_cast<int>(cl.num_blocks()), me = static_cast<int>(cl.block_rank());
     cl.sync();
@@ -177,79 +220,106 @@ struct Picker {
       uint32_t c = 0;
       u64 m = 0;
       for (int r = 0; r < C; ++r) {
-        const SampleSmem* o = cl.map_shared_rank(&S, r);
+        const FilterSmem* o = cl.map_shared_rank(&F, r);
         c += o->cnt[b];
         if (with_mass)
           m += o->part[0][b] + (static_cast<u64>(o->part[1][b]) << 15) + (static_cast<u64>(o->part[2][b]) << 30);
       }
       for (int r = 0; r < C; ++r) {
-        SampleSmem* o = cl.map_shared_rank(&S, r);
+        FilterSmem* o = cl.map_shared_rank(&F, r);
         o->tcnt[b] = c;
         if (with_mass) o->tmass[b] = m;
       }
     }
     cl.sync();
   }
-  // First bin in which the running sum of `what` reaches `target` (>= 1), with
-  // the sums before it.  Two bins a thread.
+  // Sums of the totals over all bins.
+  __device__ void whole(bool with_mass, u64* count, u64* mass) {
+    u64 c = 0, m = 0;
+    for (int b = threadIdx.x; b < kBins; b += kThreads) {
+      c += F.tcnt[b];
+      if (with_mass) m += F.tmass[b];
+    }
+    *count = block_reduce(c, S.warp_a, 0ull, AddOp());
+    *mass = with_mass ? block_reduce(m, S.warp_b, 0ull, AddOp()) : 0ull;
+  }
+  // First bin in which the running sum (of weight when by_mass, else of counts)
+  // reaches `target`, with the sums before it.  Two bins a thread.
   __device__ int border(u64 target, bool by_mass, bool with_mass, u64* before_cnt, u64* before_mass) {
     const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-    const u64 c0 = S.tcnt[2 * t], c1 = S.tcnt[2 * t + 1];
-    const u64 m0 = with_mass ? S.tmass[2 * t] : 0, m1 = with_mass ? S.tmass[2 * t + 1] : 0;
+    const u64 c0 = F.tcnt[2 * t], c1 = F.tcnt[2 * t + 1];
+    const u64 m0 = with_mass ? F.tmass[2 * t] : 0, m1 = with_mass ? F.tmass[2 * t + 1] : 0;
     u64 sc = c0 + c1, sm = m0 + m1;
     for (int d = 1; d < 32; d <<= 1) {
       const u64 a = __shfl_up_sync(0xFFFFFFFFu, sc, d), b = __shfl_up_sync(0xFFFFFFFFu, sm, d);
       if (lane >= d) sc += a, sm += b;
     }
     __syncthreads();
-    if (t == 0) S.found[0] = kBins - 1;
+    if (t == 0) F.found = kBins - 1;
     if (lane == 31) S.warp_a[w] = sc, S.warp_b[w] = sm;
     __syncthreads();
     for (int i = 0; i < w; ++i) sc += S.warp_a[i], sm += S.warp_b[i];
     // sums before bin 2t, 2t + 1 and after it
     const u64 e0c = sc - c0 - c1, e0m = sm - m0 - m1, e1c = sc - c1, e1m = sm - m1;
     const u64 a0 = by_mass ? e0m : e0c, a1 = by_mass ? e1m : e1c, a2 = by_mass ? sm : sc;
-    if (a0 < target && target <= a1) S.found[0] = 2 * t, S.result[0] = e0c, S.result[1] = e0m;
-    if (a1 < target && target <= a2) S.found[0] = 2 * t + 1, S.result[0] = e1c, S.result[1] = e1m;
+    if (a0 < target && target <= a1) F.found = 2 * t, F.result[0] = e0c, F.result[1] = e0m;
+    if (a1 < target && target <= a2) F.found = 2 * t + 1, F.result[0] = e1c, F.result[1] = e1m;
     __syncthreads();
-    const int b = S.found[0];
-    *before_cnt = S.result[0];
-    *before_mass = S.result[1];
+    const int b = F.found;
+    *before_cnt = F.result[0];
+    *before_mass = F.result[1];
     __syncthreads();
     return b;
   }
 
+  // Sends the tokens of steps [first, last] with composites in [lo, hi] to
+  // CTA 0, in any order.  At most kList by the histogram's count.
+  __device__ void gather(int first, int last, u64 lo, u64 hi) {
+    FilterSmem* head = cl.map_shared_rank(&F, 0);
+    if (threadIdx.x == 0) F.n_list = 0;
+    cl.sync();
+    for (int i = threadIdx.x; i < n; i += kThreads) {
+      const int st = step_of(x[i], row);
+      if (st < first || st > last) continue;
+      const u64 c = composite(x[i], base + i);
+      if (c < lo || c > hi) continue;
+      const u64 w = weight(x[i], row, S.table);
+      const int at = atomicAdd(&head->n_list, 1);
+      if (at < kList) {
+        head->list[at] = c;
+        head->list_w[at] = w;
+      }
+    }
+    cl.sync();
+  }
+
   // The lowest composite kept when the tokens are taken in falling order while
   // fewer than `target` of them (by_mass: of their weight) came before.
-  // tcnt / tmass hold the 1/16-octave histogram, whose whole sum is above
-  // target.  *kept_mass: the weight down to the cut.
+  // tcnt / tmass hold the histogram of steps, whose whole sum is above target.
+  // *kept_mass: the weight down to the cut (with_mass).
   __device__ u64 cut(u64 target, bool by_mass, bool with_mass, u64* kept_mass) {
     u64 bc, bm;
     const int step = border(target, by_mass, with_mass, &bc, &bm);
-    uint32_t inside = S.tcnt[step];
+    uint32_t inside = F.tcnt[step];
     u64 lo = 0, hi = ~0ull;  // composites that are still candidates
     while (inside > kList) {
       u64 mn = ~0ull, mx = 0;
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint32_t k = keys[i];
-        const u64 c = composite(k, base + i);
-        if (k && c >= lo && c <= hi && step_of(k, row) == step && weight(k, row, S.table)) {
+        const u64 c = composite(x[i], base + i);
+        if (step_of(x[i], row) == step && c >= lo && c <= hi) {
           mn = c < mn ? c : mn;
           mx = c > mx ? c : mx;
         }
       }
-      mn = cluster_reduce(cl, mn, S, S.slot_a, ~0ull, MinOp());
-      mx = cluster_reduce(cl, mx, S, S.slot_b, 0ull, MaxOp());
+      mn = cluster_reduce(cl, mn, S, S.slot_a, ~0ull, MinOp(), true);
+      mx = cluster_reduce(cl, mx, S, S.slot_b, 0ull, MaxOp(), true);
       int shift = 0;  // at least half of the bins span [mn, mx]
       while (((mx - mn) >> shift) >= kBins) ++shift;
-      clear();
+      clear(with_mass);
       for (int i = threadIdx.x; i < n; i += kThreads) {
-        const uint32_t k = keys[i];
-        const u64 c = composite(k, base + i);
-        if (k && c >= mn && c <= mx && step_of(k, row) == step) {
-          const u64 w = weight(k, row, S.table);
-          if (w) add(static_cast<int>((mx - c) >> shift), w, with_mass);
-        }
+        const u64 c = composite(x[i], base + i);
+        if (step_of(x[i], row) == step && c >= mn && c <= mx)
+          add(static_cast<int>((mx - c) >> shift), with_mass ? weight(x[i], row, S.table) : 0ull, with_mass);
       }
       total(with_mass);
       u64 c2, m2;
@@ -257,46 +327,27 @@ struct Picker {
       const int b = border(rest, by_mass, with_mass, &c2, &m2);
       bc += c2;
       bm += m2;
-      inside = S.tcnt[b];
+      inside = F.tcnt[b];
       hi = mx - (static_cast<u64>(b) << shift);
       const u64 span = (1ull << shift) - 1;
       lo = hi - mn > span ? hi - span : mn;
     }
-    // The candidates to CTA 0, in any order.
-    SampleSmem* head = cl.map_shared_rank(&S, 0);
-    if (threadIdx.x == 0) S.n_list = 0;
-    cl.sync();
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const uint32_t k = keys[i];
-      const u64 c = composite(k, base + i);
-      if (k && c >= lo && c <= hi && step_of(k, row) == step) {
-        const u64 w = weight(k, row, S.table);
-        if (w) {
-          const int at = atomicAdd(&head->n_list, 1);
-          if (at < kList) {
-            head->list[at] = c;
-            head->list_w[at] = w;
-          }
-        }
-      }
-    }
-    cl.sync();
+    gather(step, step, lo, hi);
     if (cl.block_rank() == 0) {
-      const int m = S.n_list < kList ? S.n_list : kList;
+      const int m = F.n_list < kList ? F.n_list : kList;
       u64 mine = ~0ull, w = 0;
       if (static_cast<int>(threadIdx.x) < m) {
-        const u64 c = S.list[threadIdx.x];
+        const u64 c = F.list[threadIdx.x];
         u64 rank = 0, pre = 0;
         for (int j = 0; j < m; ++j)
-          if (S.list[j] > c) ++rank, pre += S.list_w[j];
-        if ((by_mass ? bm + pre : bc + rank) < target) mine = c, w = S.list_w[threadIdx.x];
+          if (F.list[j] > c) ++rank, pre += F.list_w[j];
+        if ((by_mass ? bm + pre : bc + rank) < target) mine = c, w = F.list_w[threadIdx.x];
       }
       const u64 low = block_reduce(mine, S.warp_a, ~0ull, MinOp());
       const u64 mass = bm + block_reduce(w, S.warp_b, 0ull, AddOp());
       if (threadIdx.x < cl.num_blocks()) {
-        SampleSmem* o = cl.map_shared_rank(&S, threadIdx.x);
-        o->slot_a[0] = low;
-        o->slot_b[0] = mass;
+        cl.map_shared_rank(S.slot_a, threadIdx.x)[0] = low;
+        cl.map_shared_rank(S.slot_b, threadIdx.x)[0] = mass;
       }
     }
     cl.sync();
@@ -305,83 +356,161 @@ struct Picker {
     cl.sync();
     return low;
   }
+
+  // CTA 0: the row from its list, which holds every token down to some step.
+  // mass: the whole weight, or 0 for that of the top_k.
+  __device__ void finish(const yb_sample_args& a, int b, const Settings& s, u64 mass) {
+    const int m = F.n_list < kList ? F.n_list : kList, t = threadIdx.x;
+    const u64 c = t < m ? F.list[t] : 0ull;
+    u64 w = t < m ? F.list_w[t] : 0ull;
+    u64 rank = 0, pre = 0;
+    for (int j = 0; j < m; ++j)
+      if (F.list[j] > c) ++rank, pre += F.list_w[j];
+    if (s.top_k > 0 && rank >= static_cast<u64>(s.top_k)) w = 0;
+    if (s.top_p < 1.0f) {
+      if (!mass) mass = block_reduce(w, S.warp_a, 0ull, AddOp());
+      if (pre >= mass_target(s.top_p, mass)) w = 0;
+    }
+    if (w < s.least) w = 0;
+    const u64 all = block_reduce(w, S.warp_b, 0ull, AddOp());
+    if (t < m) F.list_w[t] = w;
+    __syncthreads();
+    if (!w) return;
+    u64 before = 0;  // kept weight of lower indexes (the composite holds ~index)
+    const uint32_t mine = static_cast<uint32_t>(c);
+    for (int j = 0; j < m; ++j)
+      if (static_cast<uint32_t>(F.list[j]) > mine) before += F.list_w[j];
+    const u64 goal = goal_of(s.u, all);
+    if (before <= goal && goal - before < w) answer(a, b, 0xFFFFFFFFu - mine, w, all);
+  }
 };
 
+// The slice into shared memory, 16 bytes a load; returns the thread's largest composite.
 template <typename T>
+__device__ __forceinline__ u64 load_slice(const T* g, float* x, int n, int head, uint32_t first) {
+  constexpr int V = 16 / sizeof(T);
+  u64 best = 0;
+  float top = -INFINITY;
+  uint32_t at = 0xFFFFFFFFu;  // of the lowest index, as a thread's indexes rise
+  auto take = [&](float v, int i) {
+    x[i] = v;
+    if (v > top) top = v, at = first + i;
+  };
+  const int vecs = (n - head) / V;
+  if (static_cast<int>(threadIdx.x) < head) take(clean(to_f(g[threadIdx.x])), threadIdx.x);
+  constexpr int U = 4;
+  for (int k0 = threadIdx.x; k0 < vecs; k0 += U * kThreads) {
+    uint4 r[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (k0 + u * kThreads < vecs)
+        r[u] = __ldcs(reinterpret_cast<const uint4*>(g + head) + k0 + u * kThreads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = k0 + u * kThreads;
+      if (k >= vecs) break;
+      const T* e = reinterpret_cast<const T*>(&r[u]);
+      float f[V];
+#pragma unroll
+      for (int d = 0; d < V; ++d) {
+        f[d] = clean(to_f(e[d]));
+        if (f[d] > top) top = f[d], at = first + head + k * V + d;
+      }
+#pragma unroll
+      for (int d = 0; d < V; d += 4)
+        *reinterpret_cast<float4*>(x + head + k * V + d) = make_float4(f[d], f[d + 1], f[d + 2], f[d + 3]);
+    }
+  }
+  best = composite(top, at);
+  const int tail = head + vecs * V;
+  if (tail + static_cast<int>(threadIdx.x) < n) {
+    const int i = tail + threadIdx.x;
+    const float v = clean(to_f(g[i]));
+    x[i] = v;
+    const u64 c = composite(v, first + i);
+    best = c > best ? c : best;
+  }
+  return best;
+}
+
+template <typename T, bool FILTER>
 __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a, int slice) {
   extern __shared__ __align__(16) uint8_t sample_raw[];
   SampleSmem& S = *reinterpret_cast<SampleSmem*>(sample_raw);
-  uint32_t* keys = reinterpret_cast<uint32_t*>(sample_raw + sizeof(SampleSmem));
+  FilterSmem& F = *reinterpret_cast<FilterSmem*>(sample_raw + sizeof(SampleSmem));
   cg::cluster_group cl = cg::this_cluster();
+  cl.barrier_arrive();  // remote shared memory may be written once all CTAs are up
   const int C = static_cast<int>(cl.num_blocks()), me = static_cast<int>(cl.block_rank());
   const int b = blockIdx.x / C;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = min(me * slice, a.V);
   const int n = min(slice, a.V - first);
-  const T* x = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.row_stride + first;
+  const T* g = static_cast<const T*>(a.logits) + static_cast<long long>(b) * a.row_stride + first;
+  // Elements before the first 16-byte boundary; shared memory is shifted so
+  // that it has its boundary at the same element.
+  const int head = min(n, static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(g) & 15u)) & 15u) / sizeof(T)));
+  float* x = reinterpret_cast<float*>(sample_raw + sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0)) +
+             ((4 - (head & 3)) & 3);
 
-  if (tid < 64) S.table[tid] = exp2(tid / 64.0);
-  u64 best = 0;
-  for (int i = tid; i < n; i += kThreads) {
-    const uint32_t k = key_of(to_f(x[i]));
-    keys[i] = k;
-    const u64 c = composite(k, first + i);
-    best = c > best ? c : best;
-  }
-  best = cluster_reduce(cl, best, S, S.slot_a, 0ull, MaxOp());
-  const uint32_t best_key = static_cast<uint32_t>(best >> 32);
   const float temp = a.temperature ? a.temperature[b] : 1.0f;
-  if (best_key == 0u || !(temp > 0.0f)) {
+  u64 best = load_slice(g, x, n, head, static_cast<uint32_t>(first));
+  if (tid < 64) {
+    const double e = exp2(tid / 64.0);
+    for (int i = 0; i < kCopies; ++i) S.table[tid * kCopies + i] = e;
+  }
+  cl.barrier_wait();
+  best = cluster_reduce(cl, best, S, S.slot_best, 0ull, MaxOp(), false);
+  const bool none = (best >> 32) == 0;
+  if (none || !(temp > 0.0f)) {
     if (me == 0 && tid == 0) {
-      a.token[b] = best_key ? static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best)) : -1;
-      if (a.logprob) a.logprob[b] = best_key ? 0.0f : -INFINITY;
+      a.token[b] = none ? -1 : static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
+      if (a.logprob) a.logprob[b] = none ? -INFINITY : 0.0f;
     }
     return;  // every CTA of the cluster, after its last remote access
   }
-  Picker P{cl, S, keys, n, static_cast<uint32_t>(first), Row()};
-  P.row.bestf = val_of(best_key);
-  P.row.best = P.row.bestf;
-  P.row.c = 1.4426950408889634074 / static_cast<double>(temp);
-  P.row.cf = static_cast<float>(fmin(P.row.c, 1e30));
+  Row row;
+  row.bestf = value_of(best);
+  row.best = widen(row.bestf);
+  row.c = 1.4426950408889634074 / static_cast<double>(temp);
+  row.cf = static_cast<float>(fmin(16.0 * row.c, 1e30));
 
-  const int top_k = a.top_k ? a.top_k[b] : 0;
-  const float top_p = a.top_p ? a.top_p[b] : 1.0f;
+  Settings s;
+  s.u = a.u[b] > 0.0f ? a.u[b] : 0.0f;
   const float min_p = a.min_p ? a.min_p[b] : 0.0f;
-  const bool use_k = top_k > 0 && top_k < a.V, use_p = top_p < 1.0f;
-  u64 cut = 1;  // keys above 0
-  if (use_k || use_p) {
-    P.clear();
-    u64 mass = 0, count = 0;
-    for (int i = tid; i < n; i += kThreads) {
-      const u64 w = weight(keys[i], P.row, S.table);
-      if (w) {
-        P.add(step_of(keys[i], P.row), w, use_p);
-        mass += w;
-        ++count;
-      }
+  s.least = min_p > 0.0f ? static_cast<u64>(fmin(rint(static_cast<double>(min_p) * kOne), kOne)) : 0ull;
+  u64 cut = 0;  // lowest composite kept
+  if constexpr (FILTER) {
+    Picker P{cl, S, F, x, n, static_cast<uint32_t>(first), row};
+    s.top_k = a.top_k ? a.top_k[b] : 0;
+    s.top_p = a.top_p ? a.top_p[b] : 1.0f;
+    if (s.top_k >= a.V) s.top_k = 0;
+    const bool use_p = s.top_p < 1.0f;
+    u64 count, mass, bc, bm;
+    if (s.top_k > 0) {
+      P.steps(false);
+      P.whole(false, &count, &mass);
+      if (static_cast<u64>(s.top_k) >= count) s.top_k = 0;  // the rest is never chosen
     }
-    P.total(use_p);
-    count = cluster_reduce(cl, count, S, S.slot_a, 0ull, AddOp());
-    if (use_p) mass = cluster_reduce(cl, mass, S, S.slot_b, 0ull, AddOp());
-    // `cut` may leave a finer histogram in tcnt / tmass; the second search
-    // needs the first one again.
-    bool fresh = true;
-    if (use_k && static_cast<u64>(top_k) < count) {
-      u64 kept = 0;
-      cut = P.cut(static_cast<u64>(top_k), false, use_p, &kept);
-      mass = kept;
-      fresh = false;
+    if (s.top_k > 0) {
+      const int step = P.border(s.top_k, false, false, &bc, &bm);
+      if (bc + F.tcnt[step] <= kList) {
+        P.gather(0, step, 0ull, ~0ull);
+        if (me == 0) P.finish(a, b, s, 0ull);
+        return;
+      }
+      if (use_p) P.steps(true);
+      cut = P.cut(s.top_k, false, use_p, &mass);
     }
     if (use_p) {
-      const u64 target = static_cast<u64>(fmax(1.0, ceil(static_cast<double>(top_p) * static_cast<double>(mass))));
+      P.steps(true);
+      if (s.top_k <= 0) P.whole(true, &count, &mass);
+      const u64 target = mass_target(s.top_p, mass);
       if (target < mass) {
-        if (!fresh) {
-          P.clear();
-          for (int i = tid; i < n; i += kThreads) {
-            const u64 w = weight(keys[i], P.row, S.table);
-            if (w) P.add(step_of(keys[i], P.row), w, true);
-          }
-          P.total(true);
+        const int step = P.border(target, true, true, &bc, &bm);
+        if (s.top_k <= 0 && bc + F.tcnt[step] <= kList) {
+          P.gather(0, step, 0ull, ~0ull);
+          if (me == 0) P.finish(a, b, s, mass);
+          return;
         }
         u64 kept = 0;
         const u64 c = P.cut(target, true, true, &kept);
@@ -389,78 +518,76 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a
       }
     }
   }
-  const u64 least = min_p > 0.0f ? static_cast<u64>(fmin(rint(static_cast<double>(min_p) * kOne), kOne)) : 0ull;
 
   // Kept weights: each warp owns a contiguous run of the slice.
   const int run = ((slice + kWarps - 1) / kWarps + 31) & ~31;
-  const int w0 = min(warp * run, n), w1 = min(w0 + run, n);
+  const float edge = cut ? value_of(cut) : -FLT_MAX;
   auto kept_weight = [&](int i) -> u64 {
-    const uint32_t k = keys[i];
-    if (composite(k, first + i) < cut) return 0ull;
-    const u64 w = weight(k, P.row, S.table);
-    return w >= least ? w : 0ull;
+    if (FILTER && (!(x[i] >= edge) || composite(x[i], first + i) < cut)) return 0ull;
+    const u64 w = weight(x[i], row, S.table);
+    return w >= s.least ? w : 0ull;
   };
   u64 sum = 0;
-  for (int i = w0 + lane; i < w1; i += 32) sum += kept_weight(i);
+  for (int i = warp * run + lane; i < min(warp * run + run, n); i += 32) sum += kept_weight(i);
   for (int m = 16; m; m >>= 1) sum += shfl_xor64(sum, m);
   __syncthreads();
   if (lane == 0) S.warp_b[warp] = sum;
   __syncthreads();
-  u64 mine = 0, before_warp = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before_warp += S.warp_b[w];
-    mine += S.warp_b[w];
-  }
-  cl.sync();
-  if (tid < C) cl.map_shared_rank(S.slot_a, tid)[me] = mine;
+  u64 mine = 0;
+  for (int w = 0; w < kWarps; ++w) mine += S.warp_b[w];
+  if (tid < C) cl.map_shared_rank(S.slot_sum, tid)[me] = mine;
   cl.sync();  // the last remote access
   u64 all = 0, before = 0;
   for (int r = 0; r < C; ++r) {
-    if (r < me) before += S.slot_a[r];
-    all += S.slot_a[r];
+    if (r < me) before += S.slot_sum[r];
+    all += S.slot_sum[r];
   }
-  float u = a.u[b];
-  u = u > 0.0f ? u : 0.0f;
-  u64 goal = static_cast<u64>(fmin(static_cast<double>(u), 1.0) * static_cast<double>(all));
-  if (goal >= all) goal = all - 1;
-  before += before_warp;
-  if (goal < before || goal - before >= sum) return;
-  goal -= before;  // the first token whose running sum exceeds it
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    const int i = i0 + lane;
-    const u64 w = i < w1 ? kept_weight(i) : 0ull;
-    u64 s = w;
+  u64 goal = goal_of(s.u, all);
+  if (goal < before || goal - before >= mine) return;  // the whole CTA
+  goal -= before;
+  int at = 0;  // the run that holds the goal
+  while (goal >= S.warp_b[at]) goal -= S.warp_b[at++];
+  // Its tokens, kThreads at a time: the first whose running sum exceeds the goal.
+  for (int i0 = at * run; i0 < min(at * run + run, n); i0 += kThreads) {
+    const int i = i0 + tid;
+    const u64 w = i < min(at * run + run, n) ? kept_weight(i) : 0ull;
+    u64 sc = w;
     for (int d = 1; d < 32; d <<= 1) {
-      const u64 o = __shfl_up_sync(0xFFFFFFFFu, s, d);
-      if (lane >= d) s += o;
+      const u64 o = __shfl_up_sync(0xFFFFFFFFu, sc, d);
+      if (lane >= d) sc += o;
     }
-    const unsigned hit = __ballot_sync(0xFFFFFFFFu, s > goal);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        a.token[b] = first + i;
-        if (a.logprob) a.logprob[b] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
-      }
-      return;
+    __syncthreads();
+    if (lane == 31) S.warp_a[warp] = sc;
+    __syncthreads();
+    u64 stage = 0;
+    for (int v = 0; v < kWarps; ++v) {
+      if (v < warp) sc += S.warp_a[v];
+      stage += S.warp_a[v];
     }
-    goal -= __shfl_sync(0xFFFFFFFFu, s, 31);
+    if (sc > goal && sc - w <= goal) answer(a, b, first + i, w, all);
+    if (stage > goal) return;
+    goal -= stage;
   }
 }
 
-template <typename T>
+template <typename T, bool FILTER>
 status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
-  // Cluster size: slices of at most kMaxSlice tokens.
+  // Slices of at most 16384 tokens; smaller ones while the CTAs do not fill
+  // the SMs twice and each thread still has four tokens.
   int C = 1;
-  while (C < kMaxCluster && (a.V + C - 1) / C > 4096) C *= 2;
+  while (C < kMaxCluster && ((a.V + C - 1) / C > 16384 ||
+                             (static_cast<long long>(a.B) * C < 2 * 148 && (a.V + C - 1) / C > 4 * kThreads)))
+    C *= 2;
   const int slice = ((a.V + C - 1) / C + 31) & ~31;
-  const size_t smem = sizeof(SampleSmem) + static_cast<size_t>(slice) * 4;
+  constexpr size_t fixed = sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0) + 16;
   static std::atomic<uint64_t> done{0};
   cudaError_t e =
-      smem_attr_once(sample_kernel<T>, static_cast<int>(sizeof(SampleSmem) + (kMaxSlice + 32) * 4), done);
+      smem_attr_once(sample_kernel<T, FILTER>, static_cast<int>(fixed + (kMaxSlice + 32) * sizeof(float)), done);
   if (e != cudaSuccess) return cuda_status(e, "sample attributes");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B) * C);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = smem;
+  cfg.dynamicSmemBytes = fixed + static_cast<size_t>(slice) * sizeof(float);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -468,7 +595,12 @@ status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return cuda_status(cudaLaunchKernelEx(&cfg, sample_kernel<T>, a, slice), "sample");
+  return cuda_status(cudaLaunchKernelEx(&cfg, sample_kernel<T, FILTER>, a, slice), "sample");
+}
+
+template <typename T>
+status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
+  return a.top_k || a.top_p ? launch_sample<T, true>(a, s) : launch_sample<T, false>(a, s);
 }
 
 }  // namespace
