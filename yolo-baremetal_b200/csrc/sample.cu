@@ -44,7 +44,7 @@ constexpr int kLive = 46 * 16;  // steps from here on weigh less than 2^-45: nev
 constexpr int kList = 512;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxSlice = YB_SAMPLE_MAX_VOCAB / kMaxCluster;
-constexpr int kCopies = 16;  // of the table, so that a warp's look-ups never share a bank
+constexpr int kCopies = 8;  // of the table: few of a warp's look-ups share a bank
 constexpr double kOne = 17592186044416.0;  // 2^44
 
 using u64 = unsigned long long;
@@ -67,39 +67,31 @@ struct alignas(16) FilterSmem {
 };
 
 // NaN, -infinity: -infinity, which is never chosen; +infinity: the largest float.
-__device__ __forceinline__ float clean(float x) {
-  return x >= -FLT_MAX ? fminf(x, FLT_MAX) + 0.0f : -INFINITY;  // -0 and 0 are equal
-}
+__device__ __forceinline__ float clean(float x) { return fminf(fmaxf(x, -INFINITY), FLT_MAX); }
 __device__ __forceinline__ u64 composite(float x, uint32_t idx) {
-  const uint32_t b = __float_as_uint(x);
+  const uint32_t b = __float_as_uint(x + 0.0f);  // -0 and 0 are equal
   const uint32_t k = b ^ ((b >> 31) ? 0xFFFFFFFFu : 0x80000000u);
-  return (static_cast<u64>(x == -INFINITY ? 0u : k) << 32) | (0xFFFFFFFFu - idx);
+  return (static_cast<u64>(k) << 32) | (0xFFFFFFFFu - idx);
 }
 __device__ __forceinline__ float value_of(u64 c) {
   const uint32_t k = static_cast<uint32_t>(c >> 32);
   return __uint_as_float(k ^ ((k >> 31) ? 0x80000000u : 0xFFFFFFFFu));
 }
 
-// fp32 -> fp64 on the integer pipe (the conversion instruction runs at a
-// quarter of the fp64 rate); subnormals become zero.
-__device__ __forceinline__ double widen(float x) {
-  const uint32_t b = __float_as_uint(x);
-  const bool tiny = (b & 0x7F800000u) == 0u;
-  const uint32_t hi = (b & 0x80000000u) | (((b & 0x7FFFFFFFu) >> 3) + (896u << 20));
-  return __hiloint2double(tiny ? 0 : static_cast<int>(hi), tiny ? 0 : static_cast<int>(b << 29));
-}
-
 struct Row {
   double best = 0, c = 0;  // largest logit, log2(e) / T
   float bestf = 0, cf = 0;
+  float floor = 0;  // tokens below weigh less than half a unit
 };
 
-// rint(2^44 2^y), y = (x - best) log2(e) / T <= 0.  2^y = 2^n 2^(j/64) 2^r with
-// |r| <= 1/128 (table-driven, after Tang 1989): the Taylor polynomial of degree
-// 4 leaves (r ln 2)^5 / 120 < 2^-44.  Ten fp64 operations, no conversion:
-// rounding to whole numbers is done by adding 1.5 2^52 and 2^52.
-__device__ __forceinline__ u64 weight(float x, const Row& r, const double* table) {
-  const double y = (widen(x) - r.best) * r.c;
+// rint(2^44 2^y), y = (x - best) log2(e) / T <= 0, as a whole fp64 number; only
+// for x >= floor.
+// 2^y = 2^n 2^(j/64) 2^r with |r| <= 1/128 (table-driven, after Tang 1989): the
+// Taylor polynomial of degree 4 leaves (r ln 2)^5 / 120 < 2^-44.  Rounding to
+// whole numbers is done by adding 1.5 2^52 and 2^52: twelve fp64 operations and
+// one conversion (they run at a quarter of the fp64 rate).
+__device__ __forceinline__ double weight_d(float x, const Row& r, const double* table) {
+  const double y = (static_cast<double>(x) - r.best) * r.c;
   const double t = fma(y, 64.0, 6755399441055744.0);
   const int k = __double2loint(t);
   const double q = fma(t - 6755399441055744.0, -0.015625, y);
@@ -107,10 +99,14 @@ __device__ __forceinline__ u64 weight(float x, const Row& r, const double* table
   p = fma(p, q, 0.24022650695910071233);                                  // ln2^2 / 2
   p = fma(p, q, 0.69314718055994530942);
   p = fma(p, q, 1.0);
-  p *= table[(k & 63) * kCopies + (threadIdx.x & (kCopies - 1))];
-  const double v = __hiloint2double(__double2hiint(p) + (((k >> 6) + 44) << 20), __double2loint(p)) + 4503599627370496.0;
-  const u64 w = static_cast<u64>(__double_as_longlong(v)) & 0xFFFFFFFFFFFFFull;
-  return y > -46.0 && x > -INFINITY ? w : 0ull;
+  p *= table[((k << 3) & (63 * kCopies)) + (threadIdx.x & (kCopies - 1))];  // 2^44 2^(j/64)
+  const double v = __hiloint2double(__double2hiint(p) + (k >> 6) * (1 << 20), __double2loint(p));
+  return (v + 4503599627370496.0) - 4503599627370496.0;
+}
+__device__ __forceinline__ u64 weight(float x, const Row& r, const double* table) {
+  if (!(x >= r.floor)) return 0ull;
+  const double v = weight_d(x, r, table) + 4503599627370496.0;
+  return static_cast<u64>(__double_as_longlong(v)) & 0xFFFFFFFFFFFFFull;
 }
 
 // Step of 1/16 octave below the maximum: rises as the logit falls.
@@ -385,26 +381,28 @@ struct Picker {
   }
 };
 
-// The slice into shared memory, 16 bytes a load; returns the thread's largest composite.
+// The slice into shared memory, 16 bytes a load; returns the thread's largest logit.
 template <typename T>
-__device__ __forceinline__ u64 load_slice(const T* g, float* x, int n, int head, uint32_t first) {
+__device__ __forceinline__ float load_slice(const T* g, float* x, int n, int head) {
   constexpr int V = 16 / sizeof(T);
-  u64 best = 0;
   float top = -INFINITY;
-  uint32_t at = 0xFFFFFFFFu;  // of the lowest index, as a thread's indexes rise
-  auto take = [&](float v, int i) {
-    x[i] = v;
-    if (v > top) top = v, at = first + i;
-  };
-  const int vecs = (n - head) / V;
-  if (static_cast<int>(threadIdx.x) < head) take(clean(to_f(g[threadIdx.x])), threadIdx.x);
+  const int vecs = (n - head) / V, tail = head + vecs * V, tid = threadIdx.x;
+  if (tid < head) {
+    top = clean(to_f(g[tid]));
+    x[tid] = top;
+  }
+  if (tail + tid < n) {
+    const float v = clean(to_f(g[tail + tid]));
+    x[tail + tid] = v;
+    top = fmaxf(top, v);
+  }
   constexpr int U = 4;
-  for (int k0 = threadIdx.x; k0 < vecs; k0 += U * kThreads) {
+  const uint4* src = reinterpret_cast<const uint4*>(g + head);
+  for (int k0 = tid; k0 < vecs; k0 += U * kThreads) {
     uint4 r[U];
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (k0 + u * kThreads < vecs)
-        r[u] = __ldcs(reinterpret_cast<const uint4*>(g + head) + k0 + u * kThreads);
+      if (k0 + u * kThreads < vecs) r[u] = __ldcs(src + k0 + u * kThreads);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int k = k0 + u * kThreads;
@@ -414,27 +412,18 @@ __device__ __forceinline__ u64 load_slice(const T* g, float* x, int n, int head,
 #pragma unroll
       for (int d = 0; d < V; ++d) {
         f[d] = clean(to_f(e[d]));
-        if (f[d] > top) top = f[d], at = first + head + k * V + d;
+        top = fmaxf(top, f[d]);
       }
 #pragma unroll
       for (int d = 0; d < V; d += 4)
         *reinterpret_cast<float4*>(x + head + k * V + d) = make_float4(f[d], f[d + 1], f[d + 2], f[d + 3]);
     }
   }
-  best = composite(top, at);
-  const int tail = head + vecs * V;
-  if (tail + static_cast<int>(threadIdx.x) < n) {
-    const int i = tail + threadIdx.x;
-    const float v = clean(to_f(g[i]));
-    x[i] = v;
-    const u64 c = composite(v, first + i);
-    best = c > best ? c : best;
-  }
-  return best;
+  return top;
 }
 
 template <typename T, bool FILTER>
-__global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a, int slice) {
+__global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const yb_sample_args a, int slice) {
   extern __shared__ __align__(16) uint8_t sample_raw[];
   SampleSmem& S = *reinterpret_cast<SampleSmem*>(sample_raw);
   FilterSmem& F = *reinterpret_cast<FilterSmem*>(sample_raw + sizeof(SampleSmem));
@@ -449,38 +438,52 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a
   // Elements before the first 16-byte boundary; shared memory is shifted so
   // that it has its boundary at the same element.
   const int head = min(n, static_cast<int>(((16u - (reinterpret_cast<uintptr_t>(g) & 15u)) & 15u) / sizeof(T)));
-  float* x = reinterpret_cast<float*>(sample_raw + sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0)) +
-             ((4 - (head & 3)) & 3);
+  const int pad = (4 - (head & 3)) & 3;
+  float* raw = reinterpret_cast<float*>(sample_raw + sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0));
+  float* x = raw + pad;
+  // Each warp sums a run of whole 32-token steps; what lies outside the slice
+  // holds -infinity.
+  const int run = (n + pad + kThreads - 1) / kThreads * 32;
 
   const float temp = a.temperature ? a.temperature[b] : 1.0f;
-  u64 best = load_slice(g, x, n, head, static_cast<uint32_t>(first));
+  const float top = load_slice(g, x, n, head);
+  if (tid < pad) raw[tid] = -INFINITY;
+  for (int i = pad + n + tid; i < kWarps * run; i += kThreads) raw[i] = -INFINITY;
   if (tid < 64) {
-    const double e = exp2(tid / 64.0);
+    const double e = kOne * exp2(tid / 64.0);
     for (int i = 0; i < kCopies; ++i) S.table[tid * kCopies + i] = e;
   }
   cl.barrier_wait();
-  best = cluster_reduce(cl, best, S, S.slot_best, 0ull, MaxOp(), false);
-  const bool none = (best >> 32) == 0;
-  if (none || !(temp > 0.0f)) {
+  u64 best = cluster_reduce(cl, composite(top, 0xFFFFFFFFu), S, S.slot_best, 0ull, MaxOp(), false);
+  const float bestf = value_of(best);
+  if (!(bestf > -INFINITY) || !(temp > 0.0f)) {
+    // The lowest index of the largest logit.
+    uint32_t at = 0xFFFFFFFFu;
+    if (bestf > -INFINITY)
+      for (int i = n - 1 - tid; i >= 0; i -= kThreads)
+        if (x[i] == bestf) at = first + i;
+    const u64 low = cluster_reduce(cl, at, S, S.slot_a, ~0ull, MinOp(), false);
     if (me == 0 && tid == 0) {
-      a.token[b] = none ? -1 : static_cast<int>(0xFFFFFFFFu - static_cast<uint32_t>(best));
-      if (a.logprob) a.logprob[b] = none ? -INFINITY : 0.0f;
+      a.token[b] = bestf > -INFINITY ? static_cast<int>(low) : -1;
+      if (a.logprob) a.logprob[b] = bestf > -INFINITY ? 0.0f : -INFINITY;
     }
     return;  // every CTA of the cluster, after its last remote access
   }
   Row row;
-  row.bestf = value_of(best);
-  row.best = widen(row.bestf);
+  row.bestf = bestf;
+  row.best = bestf;
   row.c = 1.4426950408889634074 / static_cast<double>(temp);
   row.cf = static_cast<float>(fmin(16.0 * row.c, 1e30));
+  // 2^44 2^-45.5 < 1/2 after the rounding to fp32 too (toward -infinity).
+  row.floor = __double2float_rd(fmax(row.best - 45.5 / row.c, -static_cast<double>(FLT_MAX)));
 
   Settings s;
   s.u = a.u[b] > 0.0f ? a.u[b] : 0.0f;
-  const float min_p = a.min_p ? a.min_p[b] : 0.0f;
-  s.least = min_p > 0.0f ? static_cast<u64>(fmin(rint(static_cast<double>(min_p) * kOne), kOne)) : 0ull;
   u64 cut = 0;  // lowest composite kept
   if constexpr (FILTER) {
     Picker P{cl, S, F, x, n, static_cast<uint32_t>(first), row};
+    const float min_p = a.min_p ? a.min_p[b] : 0.0f;
+    s.least = min_p > 0.0f ? static_cast<u64>(fmin(rint(static_cast<double>(min_p) * kOne), kOne)) : 0ull;
     s.top_k = a.top_k ? a.top_k[b] : 0;
     s.top_p = a.top_p ? a.top_p[b] : 1.0f;
     if (s.top_k >= a.V) s.top_k = 0;
@@ -519,16 +522,20 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a
     }
   }
 
-  // Kept weights: each warp owns a contiguous run of the slice.
-  const int run = ((slice + kWarps - 1) / kWarps + 31) & ~31;
-  const float edge = cut ? value_of(cut) : -FLT_MAX;
-  auto kept_weight = [&](int i) -> u64 {
-    if (FILTER && (!(x[i] >= edge) || composite(x[i], first + i) < cut)) return 0ull;
-    const u64 w = weight(x[i], row, S.table);
-    return w >= s.least ? w : 0ull;
+  // Kept weights of each warp's run, as whole fp64 numbers (at most 2^44 times
+  // 64 tokens a lane: exact).
+  const float edge = cut ? value_of(cut) : -INFINITY;
+  const double least = static_cast<double>(s.least);
+  auto kept = [&](int j) -> double {  // of raw[j]
+    const float v = raw[j];
+    if (FILTER && (v < edge || composite(v, first + j - pad) < cut)) return 0.0;
+    const double w = weight_d(v, row, S.table);
+    return v >= row.floor && (!FILTER || w >= least) ? w : 0.0;
   };
-  u64 sum = 0;
-  for (int i = warp * run + lane; i < min(warp * run + run, n); i += 32) sum += kept_weight(i);
+  double part = 0.0;
+#pragma unroll 8
+  for (int j = warp * run + lane; j < warp * run + run; j += 32) part += kept(j);
+  u64 sum = static_cast<u64>(part);
   for (int m = 16; m; m >>= 1) sum += shfl_xor64(sum, m);
   __syncthreads();
   if (lane == 0) S.warp_b[warp] = sum;
@@ -548,9 +555,9 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a
   int at = 0;  // the run that holds the goal
   while (goal >= S.warp_b[at]) goal -= S.warp_b[at++];
   // Its tokens, kThreads at a time: the first whose running sum exceeds the goal.
-  for (int i0 = at * run; i0 < min(at * run + run, n); i0 += kThreads) {
-    const int i = i0 + tid;
-    const u64 w = i < min(at * run + run, n) ? kept_weight(i) : 0ull;
+  for (int i0 = 0; i0 < run; i0 += kThreads) {
+    const int j = at * run + i0 + tid;
+    const u64 w = i0 + tid < run ? static_cast<u64>(kept(j)) : 0ull;
     u64 sc = w;
     for (int d = 1; d < 32; d <<= 1) {
       const u64 o = __shfl_up_sync(0xFFFFFFFFu, sc, d);
@@ -564,7 +571,7 @@ __global__ void __launch_bounds__(kThreads) sample_kernel(const yb_sample_args a
       if (v < warp) sc += S.warp_a[v];
       stage += S.warp_a[v];
     }
-    if (sc > goal && sc - w <= goal) answer(a, b, first + i, w, all);
+    if (sc > goal && sc - w <= goal) answer(a, b, first + j - pad, w, all);
     if (stage > goal) return;
     goal -= stage;
   }
@@ -579,15 +586,17 @@ status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
                              (static_cast<long long>(a.B) * C < 2 * 148 && (a.V + C - 1) / C > 4 * kThreads)))
     C *= 2;
   const int slice = ((a.V + C - 1) / C + 31) & ~31;
-  constexpr size_t fixed = sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0) + 16;
+  constexpr size_t fixed = sizeof(SampleSmem) + (FILTER ? sizeof(FilterSmem) : 0);
+  // Up to 3 elements of padding, then whole steps for every warp.
+  const auto room = [](int n) { return static_cast<size_t>((n + 3 + kThreads - 1) / kThreads * kThreads) * sizeof(float); };
   static std::atomic<uint64_t> done{0};
   cudaError_t e =
-      smem_attr_once(sample_kernel<T, FILTER>, static_cast<int>(fixed + (kMaxSlice + 32) * sizeof(float)), done);
+      smem_attr_once(sample_kernel<T, FILTER>, static_cast<int>(fixed + room(kMaxSlice)), done);
   if (e != cudaSuccess) return cuda_status(e, "sample attributes");
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(static_cast<unsigned>(a.B) * C);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = fixed + static_cast<size_t>(slice) * sizeof(float);
+  cfg.dynamicSmemBytes = fixed + room(slice);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -600,7 +609,7 @@ status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
 
 template <typename T>
 status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
-  return a.top_k || a.top_p ? launch_sample<T, true>(a, s) : launch_sample<T, false>(a, s);
+  return a.top_k || a.top_p || a.min_p ? launch_sample<T, true>(a, s) : launch_sample<T, false>(a, s);
 }
 
 }  // namespace
