@@ -30,20 +30,20 @@ def _fail(msg: str):
     raise ValueError(msg)
 
 
-def _need(t, name: str, device, dtype, shape) -> int:
-    """Data pointer of a contiguous tensor of this device, type and shape; 0 for None."""
+def _need(t, name: str, index: int, dtype, shape) -> int:
+    """Data pointer of a contiguous tensor of this CUDA device, type and shape; 0 for None."""
     if t is None:
         return 0
-    if t.dtype != dtype or t.device != device or tuple(t.shape) != shape or not t.is_contiguous():
-        _fail(f"{name}: contiguous {dtype} of shape {shape} on {device} expected, "
-              f"got {t.dtype} {tuple(t.shape)} on {t.device}")
-    return t.data_ptr()
+    if t.dtype is dtype and t.shape == shape and t.get_device() == index and t.is_contiguous():
+        return t.data_ptr()
+    _fail(f"{name}: contiguous {dtype} of shape {tuple(shape)} on cuda:{index} expected, "
+          f"got {t.dtype} {tuple(t.shape)} on {t.device}")
 
 
-def _heads(t, name: str, device, dtype, shape) -> tuple:
+def _heads(t, name: str, index: int, dtype, shape) -> tuple:
     """Strides (batch, row, head) of a [B, rows, heads, D] tensor whose last dimension is contiguous."""
-    if t.dtype != dtype or t.device != device or t.shape != shape:
-        _fail(f"{name}: {dtype} of shape {tuple(shape)} on {device} expected, "
+    if t.dtype is not dtype or t.shape != shape or t.get_device() != index:
+        _fail(f"{name}: {dtype} of shape {tuple(shape)} on cuda:{index} expected, "
               f"got {t.dtype} {tuple(t.shape)} on {t.device}")
     s = t.stride()
     if s[3] != 1 and shape[3] > 1:
@@ -53,34 +53,30 @@ def _heads(t, name: str, device, dtype, shape) -> tuple:
 
 def _writable(t, name: str) -> None:
     """Refuses an output whose elements share memory with one another."""
-    for n, s in zip(t.shape, t.stride()):
-        if n > 1 and s == 0:
-            _fail(f"{name}: an output must not be expanded")
+    if not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+        _fail(f"{name}: an output must not be expanded")
 
 
-def _cuda(t, name: str):
+def _cuda(t, name: str) -> int:
     if not t.is_cuda:
         _fail(f"{name}: a CUDA tensor expected, got {t.device}")
-    return t.device
+    return t.get_device()
 
 
-class _On:
-    """Makes the tensors' device the current one for a call, where it is not."""
+def _public_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
 
-    __slots__ = ("guard", "stream")
 
-    def __init__(self, device):
-        self.guard = None if torch.cuda.current_device() == device.index else torch.cuda.device(device)
-        self.stream = torch.cuda.current_stream(device).cuda_stream
+# The handle of the current stream without a Python stream object around it.
+_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _public_stream)
 
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
 
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _call(f, args, index: int) -> int:
+    """Calls an entry point that runs on the current device, on the tensors' device and stream."""
+    if torch.cuda.current_device() == index:
+        return f(args, _stream(index))
+    with torch.cuda.device(index):
+        return f(args, _stream(index))
 
 
 class Attention:
@@ -106,6 +102,7 @@ class Attention:
             if device.index is None:
                 device = torch.device("cuda", torch.cuda.current_device())
         self.device = device
+        self._scratch = {}  # bytes by (B, Sq, Sk)
         self._h = C.c_void_p()
         yb.check(yb.lib().yb_attn_create(self.device.index, C.byref(self._h)), "yb_attn_create")
 
@@ -129,36 +126,37 @@ class Attention:
 
         q_len, k_len, prefix int32 [B]; key_range int32 [B, Sq, 2]; slopes float32 [heads].  Rows past q_len keep
         what `out` holds (zeros where it is allocated here)."""
-        dev, dt = self.device, self.dtype
-        if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+        index, dt = self.device.index, self.dtype
+        if q.dim() != 4 or k.dim() != 4:
             _fail("attention: q, k and v have four dimensions")
-        B, Sq = q.shape[:2]
+        B, Sq, _, _ = q.shape
         Sk = k.shape[1]
-        qs = _heads(q, "q", dev, dt, (B, Sq, self.heads, self.head_dim))
-        ks = _heads(k, "k", dev, dt, (B, Sk, self.kv_heads, self.head_dim))
-        vs = _heads(v, "v", dev, dt, k.shape)
+        qs = _heads(q, "q", index, dt, (B, Sq, self.heads, self.head_dim))
+        ks = _heads(k, "k", index, dt, (B, Sk, self.kv_heads, self.head_dim))
+        vs = _heads(v, "v", index, dt, k.shape)
         if out is None:
             make = torch.empty if q_len is None else torch.zeros
-            out = make((B, Sq, self.heads, self.head_dim), dtype=dt, device=dev)
-        os = _heads(out, "out", dev, dt, q.shape)
+            out = make((B, Sq, self.heads, self.head_dim), dtype=dt, device=self.device)
+        os = _heads(out, "out", index, dt, q.shape)
         _writable(out, "out")
         i32 = torch.int32
         args = _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(),
-                          _need(q_len, "q_len", dev, i32, (B,)), _need(k_len, "k_len", dev, i32, (B,)),
-                          _need(prefix, "prefix", dev, i32, (B,)),
-                          _need(key_range, "key_range", dev, i32, (B, Sq, 2)),
-                          _need(slopes, "slopes", dev, torch.float32, (self.heads,)), *qs, *ks, *vs, *os,
+                          _need(q_len, "q_len", index, i32, (B,)), _need(k_len, "k_len", index, i32, (B,)),
+                          _need(prefix, "prefix", index, i32, (B,)),
+                          _need(key_range, "key_range", index, i32, (B, Sq, 2)),
+                          _need(slopes, "slopes", index, torch.float32, (self.heads,)), *qs, *ks, *vs, *os,
                           _DTYPE[dt], B, Sq, Sk, self.heads, self.kv_heads, self.head_dim, self.causal, self.scale,
                           self.cap)
-        L = yb.lib()
-        n = C.c_size_t()
-        st = L.yb_attn_workspace(self._h, args, C.byref(n))
-        if st:
-            yb.check(st, "yb_attn_workspace")
+        n = self._scratch.get((B, Sq, Sk))
+        if n is None:
+            size = C.c_size_t()
+            yb.check(yb.lib().yb_attn_workspace(self._h, args, C.byref(size)), "yb_attn_workspace")
+            n = size.value
+            if len(self._scratch) < 4096:
+                self._scratch[(B, Sq, Sk)] = n
         # Scratch from torch's allocator: its own for each call in flight and for each captured graph.
-        ws = torch.empty(n.value, dtype=torch.uint8, device=dev) if n.value else None
-        st = L.yb_attn_run(self._h, args, ws.data_ptr() if n.value else None, n.value,
-                           torch.cuda.current_stream(dev).cuda_stream)
+        ws = torch.empty(n, dtype=torch.uint8, device=self.device) if n else None
+        st = yb.lib().yb_attn_run(self._h, args, ws.data_ptr() if n else None, n, _stream(index))
         if st:
             yb.check(st, "yb_attn_run")
         return out
@@ -171,7 +169,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, q_out=None, k_out=None, v=N
     k_out (and v_out) [B, rows, Hkv, D] may be caches, written from row start[b] on.  Weights float32 [D] or None,
     inv_freq float64 [R/2] (R rotated dimensions), start and length int32 [B], positions int32 [B, S].
     Returns (q_out, k_out)."""
-    dev, dt = _cuda(q, "q"), q.dtype
+    dev, dt, where = _cuda(q, "q"), q.dtype, q.device
     if dt not in _DTYPE:
         _fail(f"qk_norm_rope: float32, float16 or bfloat16, got {dt}")
     if q.dim() != 4 or k.dim() != 4:
@@ -184,11 +182,11 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, q_out=None, k_out=None, v=N
         _fail("qk_norm_rope: v and v_out go together")
     make = torch.empty if length is None else torch.zeros
     if q_out is None:
-        q_out = make((B, S, Hq, D), dtype=dt, device=dev)
+        q_out = make((B, S, Hq, D), dtype=dt, device=where)
     if k_out is None:
         if start is not None:
             _fail("qk_norm_rope: start needs k_out")
-        k_out = make((B, S, Hkv, D), dtype=dt, device=dev)
+        k_out = make((B, S, Hkv, D), dtype=dt, device=where)
     if k_out.dim() != 4:
         _fail("qk_norm_rope: k_out has four dimensions")
     rows = k_out.shape[1]
@@ -212,8 +210,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, q_out=None, k_out=None, v=N
                     _need(length, "length", dev, i32, (B,)), _need(positions, "positions", dev, i32, (B, S)),
                     *qs, *ks, *vs, *qos, *kos, *vos, _DTYPE[dt], B, S, rows, Hq, Hkv, D, 2 * half, bool(interleaved),
                     eps, weight_add)
-    with _On(dev) as stream:
-        st = yb.lib().yb_qk_norm_rope(args, stream)
+    st = _call(yb.lib().yb_qk_norm_rope, args, dev)
     if st:
         yb.check(st, "yb_qk_norm_rope")
     return q_out, k_out
@@ -223,7 +220,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     """yb_sample: one token for each row of logits [B, V] at the random numbers u [B] in [0, 1).
 
     temperature, top_p, min_p float32 [B], top_k int32 [B].  Returns (token int32 [B], logprob float32 [B])."""
-    dev, dt = _cuda(logits, "logits"), logits.dtype
+    dev, dt, where = _cuda(logits, "logits"), logits.dtype, logits.device
     if dt not in _DTYPE:
         _fail(f"sample: float32, float16 or bfloat16, got {dt}")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
@@ -233,16 +230,15 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     if u is None:
         _fail("sample: u is needed")
     if token is None:
-        token = torch.empty(B, dtype=i32, device=dev)
+        token = torch.empty(B, dtype=i32, device=where)
     if logprob is None:
-        logprob = torch.empty(B, dtype=f32, device=dev)
+        logprob = torch.empty(B, dtype=f32, device=where)
     args = _SAMPLE.pack(logits.data_ptr(), _need(u, "u", dev, f32, (B,)),
                         _need(temperature, "temperature", dev, f32, (B,)), _need(top_k, "top_k", dev, i32, (B,)),
                         _need(top_p, "top_p", dev, f32, (B,)), _need(min_p, "min_p", dev, f32, (B,)),
                         _need(token, "token", dev, i32, (B,)), _need(logprob, "logprob", dev, f32, (B,)),
                         logits.stride(0), _DTYPE[dt], B, V)
-    with _On(dev) as stream:
-        st = yb.lib().yb_sample(args, stream)
+    st = _call(yb.lib().yb_sample, args, dev)
     if st:
         yb.check(st, "yb_sample")
     return token, logprob
