@@ -59,11 +59,19 @@ struct alignas(16) FilterSmem {
   uint32_t tcnt[kBins];
   uint32_t cnt[kBins];      // own slice; the weights' sums in three 15-bit parts
   uint32_t part[3][kBins];  // (2^15 tokens of a slice: 30 bits each)
-  u64 list[kList];
-  u64 list_w[kList];
+  union {
+    struct {  // totalling: each CTA's sums of this CTA's share of the bins
+      u64 mass[kBins];
+      uint32_t cnt[kBins];
+    } in;
+    struct {  // ranking; in CTA 0 `list` takes the tokens of all
+      u64 list[kList];
+      u64 own[kList];
+    } l;
+  };
   u64 result[2];
-  int found;
-  int n_list;
+  u64 rank_sum[2];
+  int found, n_own, base, n_list;
 };
 
 // NaN, -infinity: -infinity, which is never chosen; +infinity: the largest float.
@@ -134,9 +142,6 @@ struct MaxOp {
 struct MinOp {
   __device__ u64 operator()(u64 a, u64 b) const { return a < b ? a : b; }
 };
-struct AddOp {
-  __device__ u64 operator()(u64 a, u64 b) const { return a + b; }
-};
 
 // The same value in every thread of the cluster.  The slots' earlier readers
 // are done once the caller is behind a cluster barrier of its own (`sync`).
@@ -171,6 +176,12 @@ __device__ __forceinline__ void answer(const yb_sample_args& a, int b, uint32_t 
   if (a.logprob) a.logprob[b] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
 }
 
+// Bins 2 t and 2 t + 1 of thread t: what lies before each, and the sums of all.
+struct Bins {
+  u64 c[3], m[3];  // counts and weights before bin 2 t, before 2 t + 1, after it
+  u64 all_c, all_m;
+};
+
 struct Picker {
   cg::cluster_group& cl;
   SampleSmem& S;
@@ -197,52 +208,51 @@ struct Picker {
       if (p2) atomicAdd(&F.part[2][b], p2);
     }
   }
-  __device__ void steps(bool with_mass) {
+  __device__ Bins steps(bool with_mass) {
     clear(with_mass);
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int b = step_of(x[i], row);
-      if (b < kLive) add(b, with_mass ? weight(x[i], row, S.table) : 0ull, with_mass);
+      const float v = x[i];
+      const int b = step_of(v, row);
+      if (b < kLive) add(b, with_mass ? weight(v, row, S.table) : 0ull, with_mass);
     }
-    total(with_mass);
+    return total(with_mass);
   }
   // Cluster totals of the histogram into tcnt, tmass of every CTA: each CTA
-  // sums its share of the bins and writes them to all.
-  __device__ void total(bool with_mass) {
-    const int C = static_cast<int>(cl.num_blocks()), me = static_cast<int>(cl.block_rank());
-    cl.sync();
+  // sends the bins of another's share there, sums its own share and sends the
+  // sums to all (remote stores, which nobody waits for one by one).
+  __device__ Bins total(bool with_mass) {
+    const int C = static_cast<int>(cl.num_blocks()), me = static_cast<int>(cl.block_rank()), t = threadIdx.x;
     const int share = kBins / C;
-    for (int i = threadIdx.x; i < share; i += kThreads) {
-      const int b = me * share + i;
+    __syncthreads();
+    for (int b = t; b < kBins; b += kThreads) {
+      FilterSmem* o = cl.map_shared_rank(&F, b / share);
+      const int at = me * share + (b & (share - 1));
+      o->in.cnt[at] = F.cnt[b];
+      if (with_mass)
+        o->in.mass[at] = F.part[0][b] + (static_cast<u64>(F.part[1][b]) << 15) + (static_cast<u64>(F.part[2][b]) << 30);
+    }
+    cl.sync();
+    const int group = max(1, kThreads / share);  // threads that share a bin and split the receivers
+    for (int i = t & (share - 1); i < share; i += kThreads) {
       uint32_t c = 0;
       u64 m = 0;
-      for (int r = 0; r < C; ++r) {
-        const FilterSmem* o = cl.map_shared_rank(&F, r);
-        c += o->cnt[b];
-        if (with_mass)
-          m += o->part[0][b] + (static_cast<u64>(o->part[1][b]) << 15) + (static_cast<u64>(o->part[2][b]) << 30);
-      }
-      for (int r = 0; r < C; ++r) {
+#pragma unroll
+      for (int r = 0; r < kMaxCluster; ++r)
+        if (r < C) {
+          c += F.in.cnt[r * share + i];
+          if (with_mass) m += F.in.mass[r * share + i];
+        }
+      for (int r = t / share; r < C; r += group) {
         FilterSmem* o = cl.map_shared_rank(&F, r);
-        o->tcnt[b] = c;
-        if (with_mass) o->tmass[b] = m;
+        o->tcnt[me * share + i] = c;
+        if (with_mass) o->tmass[me * share + i] = m;
       }
+      if (share > kThreads && i + kThreads >= share) break;
     }
     cl.sync();
-  }
-  // Sums of the totals over all bins.
-  __device__ void whole(bool with_mass, u64* count, u64* mass) {
-    u64 c = 0, m = 0;
-    for (int b = threadIdx.x; b < kBins; b += kThreads) {
-      c += F.tcnt[b];
-      if (with_mass) m += F.tmass[b];
-    }
-    *count = block_reduce(c, S.warp_a, 0ull, AddOp());
-    *mass = with_mass ? block_reduce(m, S.warp_b, 0ull, AddOp()) : 0ull;
-  }
-  // First bin in which the running sum (of weight when by_mass, else of counts)
-  // reaches `target`, with the sums before it.  Two bins a thread.
-  __device__ int border(u64 target, bool by_mass, bool with_mass, u64* before_cnt, u64* before_mass) {
-    const int t = threadIdx.x, lane = t & 31, w = t >> 5;
+    // Running sums.
+    const int lane = t & 31, w = t >> 5;
     const u64 c0 = F.tcnt[2 * t], c1 = F.tcnt[2 * t + 1];
     const u64 m0 = with_mass ? F.tmass[2 * t] : 0, m1 = with_mass ? F.tmass[2 * t + 1] : 0;
     u64 sc = c0 + c1, sm = m0 + m1;
@@ -250,52 +260,132 @@ struct Picker {
       const u64 a = __shfl_up_sync(0xFFFFFFFFu, sc, d), b = __shfl_up_sync(0xFFFFFFFFu, sm, d);
       if (lane >= d) sc += a, sm += b;
     }
-    __syncthreads();
-    if (t == 0) F.found = kBins - 1;
     if (lane == 31) S.warp_a[w] = sc, S.warp_b[w] = sm;
     __syncthreads();
-    for (int i = 0; i < w; ++i) sc += S.warp_a[i], sm += S.warp_b[i];
-    // sums before bin 2t, 2t + 1 and after it
-    const u64 e0c = sc - c0 - c1, e0m = sm - m0 - m1, e1c = sc - c1, e1m = sm - m1;
-    const u64 a0 = by_mass ? e0m : e0c, a1 = by_mass ? e1m : e1c, a2 = by_mass ? sm : sc;
-    if (a0 < target && target <= a1) F.found = 2 * t, F.result[0] = e0c, F.result[1] = e0m;
-    if (a1 < target && target <= a2) F.found = 2 * t + 1, F.result[0] = e1c, F.result[1] = e1m;
+    Bins r;
+    r.all_c = r.all_m = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      const u64 a = S.warp_a[i], b = S.warp_b[i];
+      if (i < w) sc += a, sm += b;
+      r.all_c += a;
+      r.all_m += b;
+    }
+    r.c[0] = sc - c0 - c1, r.c[1] = sc - c1, r.c[2] = sc;
+    r.m[0] = sm - m0 - m1, r.m[1] = sm - m1, r.m[2] = sm;
+    return r;
+  }
+  // First bin in which the running sum (of weight when by_mass, else of counts)
+  // reaches `target` (at most the whole), with the sums before it.
+  __device__ int border(const Bins& r, u64 target, bool by_mass, u64* before_cnt, u64* before_mass) {
+    const int t = threadIdx.x;
+    if (t == 0) F.found = kBins - 1;
     __syncthreads();
-    const int b = F.found;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      if ((by_mass ? r.m[i] : r.c[i]) < target && target <= (by_mass ? r.m[i + 1] : r.c[i + 1])) {
+        F.found = 2 * t + i;
+        F.result[0] = r.c[i];
+        F.result[1] = r.m[i];
+      }
+    __syncthreads();
     *before_cnt = F.result[0];
     *before_mass = F.result[1];
-    __syncthreads();
-    return b;
+    return F.found;
   }
 
-  // Sends the tokens of steps [first, last] with composites in [lo, hi] to
-  // CTA 0, in any order.  At most kList by the histogram's count.
+  // The tokens of steps [first, last] with composites in [lo, hi] to CTA 0's
+  // list, in any order; at most kList by the histogram's count.  n_own and CTA
+  // 0's n_list are zero.
   __device__ void gather(int first, int last, u64 lo, u64 hi) {
     FilterSmem* head = cl.map_shared_rank(&F, 0);
-    if (threadIdx.x == 0) F.n_list = 0;
-    cl.sync();
+#pragma unroll 4
     for (int i = threadIdx.x; i < n; i += kThreads) {
-      const int st = step_of(x[i], row);
+      const float v = x[i];
+      const int st = step_of(v, row);
       if (st < first || st > last) continue;
-      const u64 c = composite(x[i], base + i);
+      const u64 c = composite(v, base + i);
       if (c < lo || c > hi) continue;
-      const u64 w = weight(x[i], row, S.table);
-      const int at = atomicAdd(&head->n_list, 1);
-      if (at < kList) {
-        head->list[at] = c;
-        head->list_w[at] = w;
-      }
+      const int at = atomicAdd(&F.n_own, 1);
+      if (at < kList) F.l.own[at] = c;
     }
+    __syncthreads();
+    const int m = min(F.n_own, kList);
+    if (threadIdx.x == 0) F.base = m ? atomicAdd(&head->n_list, m) : 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < m; i += kThreads)
+      if (F.base + i < kList) head->l.list[F.base + i] = F.l.own[i];
     cl.sync();
+  }
+
+  // Sorts the values of the first m threads, all distinct and above 0, falling;
+  // the others get 0.  Up to 128 of them by counting, four threads a value (0.6
+  // us for 60 values, the network below 1.4); more by a bitonic network (2.7 us
+  // for 250, counting 4).
+  __device__ u64 sort(u64 v, int m) {
+    const int t = threadIdx.x;
+    if (m <= kThreads / 4) {
+      __syncthreads();
+      F.l.own[t] = t < m ? v : 0ull;
+      __syncthreads();
+      const u64 mine = F.l.own[t >> 2];
+      int rank = 0;
+#pragma unroll 4
+      for (int j = t & 3; j < m; j += 4) rank += F.l.own[j] > mine;
+      rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 1);
+      rank += __shfl_xor_sync(0xFFFFFFFFu, rank, 2);
+      __syncthreads();
+      if ((t & 3) == 0 && (t >> 2) < m) F.l.own[rank] = mine;
+      __syncthreads();
+      return t < m ? F.l.own[t] : 0ull;
+    }
+    const int size = 1 << (32 - __clz(m - 1));
+    if (t >= m) v = 0ull;
+    for (int k = 2; k <= size; k <<= 1)
+      for (int j = k >> 1; j; j >>= 1) {
+        u64 o;
+        if (j < 32) {
+          o = shfl_xor64(v, j);
+        } else {
+          __syncthreads();
+          F.l.own[t] = v;
+          __syncthreads();
+          o = F.l.own[t ^ j];
+        }
+        const bool up = (t & k) != 0, low = (t & j) == 0;  // falling runs where !up
+        v = (low != up) == (v > o) ? v : o;
+      }
+    return v;
+  }
+  // Running sum over the block's threads, this one included.
+  __device__ u64 scan(u64 v) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    for (int d = 1; d < 32; d <<= 1) {
+      const u64 o = __shfl_up_sync(0xFFFFFFFFu, v, d);
+      if (lane >= d) v += o;
+    }
+    __syncthreads();
+    if (lane == 31) S.warp_a[w] = v;
+    __syncthreads();
+    for (int i = 0; i < kWarps; ++i)
+      if (i < w) v += S.warp_a[i];
+    return v;
+  }
+  // CTA 0: its list in falling order, one token a thread, with their weights
+  // and running sums; returns the list's length.
+  __device__ int ranked(u64* c, u64* w, u64* sum) {
+    const int m = min(F.n_list, kList), t = threadIdx.x;
+    *c = sort(t < m ? F.l.list[t] : 0ull, m);
+    *w = t < m ? weight(value_of(*c), row, S.table) : 0ull;
+    *sum = scan(*w);
+    return m;
   }
 
   // The lowest composite kept when the tokens are taken in falling order while
-  // fewer than `target` of them (by_mass: of their weight) came before.
-  // tcnt / tmass hold the histogram of steps, whose whole sum is above target.
-  // *kept_mass: the weight down to the cut (with_mass).
-  __device__ u64 cut(u64 target, bool by_mass, bool with_mass, u64* kept_mass) {
-    u64 bc, bm;
-    const int step = border(target, by_mass, with_mass, &bc, &bm);
+  // fewer than `target` of them (by_mass: of their weight) came before; `step`
+  // holds the border, bc and bm are the sums before it.  *kept_mass: the
+  // weight down to the cut (with_mass).
+  __device__ u64 cut(int step, u64 bc, u64 bm, u64 target, bool by_mass, bool with_mass, u64* kept_mass) {
     uint32_t inside = F.tcnt[step];
     u64 lo = 0, hi = ~0ull;  // composites that are still candidates
     while (inside > kList) {
@@ -317,10 +407,9 @@ struct Picker {
         if (step_of(x[i], row) == step && c >= mn && c <= mx)
           add(static_cast<int>((mx - c) >> shift), with_mass ? weight(x[i], row, S.table) : 0ull, with_mass);
       }
-      total(with_mass);
+      const Bins r = total(with_mass);
       u64 c2, m2;
-      const u64 rest = target - (by_mass ? bm : bc);
-      const int b = border(rest, by_mass, with_mass, &c2, &m2);
+      const int b = border(r, target - (by_mass ? bm : bc), by_mass, &c2, &m2);
       bc += c2;
       bm += m2;
       inside = F.tcnt[b];
@@ -330,54 +419,48 @@ struct Picker {
     }
     gather(step, step, lo, hi);
     if (cl.block_rank() == 0) {
-      const int m = F.n_list < kList ? F.n_list : kList;
-      u64 mine = ~0ull, w = 0;
-      if (static_cast<int>(threadIdx.x) < m) {
-        const u64 c = F.list[threadIdx.x];
-        u64 rank = 0, pre = 0;
-        for (int j = 0; j < m; ++j)
-          if (F.list[j] > c) ++rank, pre += F.list_w[j];
-        if ((by_mass ? bm + pre : bc + rank) < target) mine = c, w = F.list_w[threadIdx.x];
-      }
-      const u64 low = block_reduce(mine, S.warp_a, ~0ull, MinOp());
-      const u64 mass = bm + block_reduce(w, S.warp_b, 0ull, AddOp());
-      if (threadIdx.x < cl.num_blocks()) {
-        cl.map_shared_rank(S.slot_a, threadIdx.x)[0] = low;
-        cl.map_shared_rank(S.slot_b, threadIdx.x)[0] = mass;
+      u64 c, w, sum;
+      const int m = ranked(&c, &w, &sum), t = threadIdx.x;
+      const bool keep = t < m && (by_mass ? bm + sum - w : bc + t) < target;
+      const int last = __syncthreads_count(keep) - 1;
+      if (t == last) F.rank_sum[0] = c, F.rank_sum[1] = bm + sum;
+      if (t == 0) F.n_list = 0;
+      __syncthreads();
+      if (t < static_cast<int>(cl.num_blocks())) {
+        cl.map_shared_rank(S.slot_a, t)[0] = F.rank_sum[0];
+        cl.map_shared_rank(S.slot_b, t)[0] = F.rank_sum[1];
       }
     }
+    if (threadIdx.x == 0) F.n_own = 0;
     cl.sync();
-    const u64 low = S.slot_a[0];
     *kept_mass = S.slot_b[0];
-    cl.sync();
-    return low;
+    return S.slot_a[0];
   }
 
   // CTA 0: the row from its list, which holds every token down to some step.
-  // mass: the whole weight, or 0 for that of the top_k.
+  // mass: the whole weight, when there is no top_k.  What the filters keep is
+  // the beginning of the falling order.
   __device__ void finish(const yb_sample_args& a, int b, const Settings& s, u64 mass) {
-    const int m = F.n_list < kList ? F.n_list : kList, t = threadIdx.x;
-    const u64 c = t < m ? F.list[t] : 0ull;
-    u64 w = t < m ? F.list_w[t] : 0ull;
-    u64 rank = 0, pre = 0;
-    for (int j = 0; j < m; ++j)
-      if (F.list[j] > c) ++rank, pre += F.list_w[j];
-    if (s.top_k > 0 && rank >= static_cast<u64>(s.top_k)) w = 0;
-    if (s.top_p < 1.0f) {
-      if (!mass) mass = block_reduce(w, S.warp_a, 0ull, AddOp());
-      if (pre >= mass_target(s.top_p, mass)) w = 0;
+    u64 c, w, sum;
+    const int m = ranked(&c, &w, &sum), t = threadIdx.x;
+    if (s.top_k > 0) {
+      if (t == s.top_k - 1) F.rank_sum[0] = sum;
+      __syncthreads();
+      mass = F.rank_sum[0];
     }
-    if (w < s.least) w = 0;
-    const u64 all = block_reduce(w, S.warp_b, 0ull, AddOp());
-    if (t < m) F.list_w[t] = w;
+    const bool keep = t < m && (s.top_k <= 0 || t < s.top_k) &&
+                      (!(s.top_p < 1.0f) || sum - w < mass_target(s.top_p, mass)) && w >= s.least;
+    const int kept = __syncthreads_count(keep);
+    if (t == kept - 1) F.rank_sum[1] = sum;
+    // By rising index: the composite's low half is ~index.
+    F.l.list[t] = w;
+    const u64 by_index = sort(t < kept ? (c << 32) | static_cast<uint32_t>(t) : 0ull, kept);
     __syncthreads();
-    if (!w) return;
-    u64 before = 0;  // kept weight of lower indexes (the composite holds ~index)
-    const uint32_t mine = static_cast<uint32_t>(c);
-    for (int j = 0; j < m; ++j)
-      if (static_cast<uint32_t>(F.list[j]) > mine) before += F.list_w[j];
+    const u64 all = F.rank_sum[1];
+    const u64 wi = t < kept ? F.l.list[static_cast<uint32_t>(by_index)] : 0ull;
+    const u64 upto = scan(wi);
     const u64 goal = goal_of(s.u, all);
-    if (before <= goal && goal - before < w) answer(a, b, 0xFFFFFFFFu - mine, w, all);
+    if (t < kept && upto > goal && upto - wi <= goal) answer(a, b, 0xFFFFFFFFu - static_cast<uint32_t>(by_index >> 32), wi, all);
   }
 };
 
@@ -447,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
 
   const float temp = a.temperature ? a.temperature[b] : 1.0f;
   const float top = load_slice(g, x, n, head);
+  if (FILTER && tid == 0) F.n_own = F.n_list = 0;
   if (tid < pad) raw[tid] = -INFINITY;
   for (int i = pad + n + tid; i < kWarps * run; i += kThreads) raw[i] = -INFINITY;
   if (tid < 64) {
@@ -488,35 +572,39 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
     s.top_p = a.top_p ? a.top_p[b] : 1.0f;
     if (s.top_k >= a.V) s.top_k = 0;
     const bool use_p = s.top_p < 1.0f;
-    u64 count, mass, bc, bm;
+    u64 mass = 0, bc, bm;
+    bool have_k = false;
     if (s.top_k > 0) {
-      P.steps(false);
-      P.whole(false, &count, &mass);
-      if (static_cast<u64>(s.top_k) >= count) s.top_k = 0;  // the rest is never chosen
-    }
-    if (s.top_k > 0) {
-      const int step = P.border(s.top_k, false, false, &bc, &bm);
-      if (bc + F.tcnt[step] <= kList) {
-        P.gather(0, step, 0ull, ~0ull);
-        if (me == 0) P.finish(a, b, s, 0ull);
-        return;
+      Bins r = P.steps(false);
+      if (static_cast<u64>(s.top_k) < r.all_c) {  // else the rest is never chosen
+        int step = P.border(r, s.top_k, false, &bc, &bm);
+        if (bc + F.tcnt[step] <= kList) {
+          P.gather(0, step, 0ull, ~0ull);
+          if (me == 0) P.finish(a, b, s, 0ull);
+          return;
+        }
+        if (use_p) {
+          r = P.steps(true);
+          step = P.border(r, s.top_k, false, &bc, &bm);
+        }
+        cut = P.cut(step, bc, bm, s.top_k, false, use_p, &mass);
+        have_k = true;
       }
-      if (use_p) P.steps(true);
-      cut = P.cut(s.top_k, false, use_p, &mass);
     }
     if (use_p) {
-      P.steps(true);
-      if (s.top_k <= 0) P.whole(true, &count, &mass);
+      const Bins r = P.steps(true);
+      if (!have_k) mass = r.all_m;
       const u64 target = mass_target(s.top_p, mass);
       if (target < mass) {
-        const int step = P.border(target, true, true, &bc, &bm);
-        if (s.top_k <= 0 && bc + F.tcnt[step] <= kList) {
+        const int step = P.border(r, target, true, &bc, &bm);
+        if (!have_k && bc + F.tcnt[step] <= kList) {
           P.gather(0, step, 0ull, ~0ull);
+          s.top_k = 0;
           if (me == 0) P.finish(a, b, s, mass);
           return;
         }
         u64 kept = 0;
-        const u64 c = P.cut(target, true, true, &kept);
+        const u64 c = P.cut(step, bc, bm, target, true, true, &kept);
         cut = c > cut ? c : cut;
       }
     }
@@ -554,26 +642,29 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
   goal -= before;
   int at = 0;  // the run that holds the goal
   while (goal >= S.warp_b[at]) goal -= S.warp_b[at++];
-  // Its tokens, kThreads at a time: the first whose running sum exceeds the goal.
-  for (int i0 = 0; i0 < run; i0 += kThreads) {
-    const int j = at * run + i0 + tid;
-    const u64 w = i0 + tid < run ? static_cast<u64>(kept(j)) : 0ull;
-    u64 sc = w;
-    for (int d = 1; d < 32; d <<= 1) {
-      const u64 o = __shfl_up_sync(0xFFFFFFFFu, sc, d);
-      if (lane >= d) sc += o;
+  // Its tokens, a few neighbours a thread: the first whose running sum exceeds the goal.
+  const int per = (run + kThreads - 1) / kThreads;
+  const int j0 = at * run + min(tid * per, run), j1 = at * run + min(tid * per + per, run);
+  u64 own = 0;
+  for (int j = j0; j < j1; ++j) own += static_cast<u64>(kept(j));
+  u64 upto = own;
+  for (int d = 1; d < 32; d <<= 1) {
+    const u64 o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += o;
+  }
+  if (lane == 31) S.warp_a[warp] = upto;
+  __syncthreads();
+  for (int v = 0; v < kWarps; ++v)
+    if (v < warp) upto += S.warp_a[v];
+  if (upto <= goal || upto - own > goal) return;
+  u64 run_sum = upto - own;
+  for (int j = j0; j < j1; ++j) {
+    const u64 w = static_cast<u64>(kept(j));
+    run_sum += w;
+    if (run_sum > goal) {
+      answer(a, b, first + j - pad, w, all);
+      return;
     }
-    __syncthreads();
-    if (lane == 31) S.warp_a[warp] = sc;
-    __syncthreads();
-    u64 stage = 0;
-    for (int v = 0; v < kWarps; ++v) {
-      if (v < warp) sc += S.warp_a[v];
-      stage += S.warp_a[v];
-    }
-    if (sc > goal && sc - w <= goal) answer(a, b, first + j - pad, w, all);
-    if (stage > goal) return;
-    goal -= stage;
   }
 }
 
