@@ -50,8 +50,10 @@ namespace yb {
 namespace {
 
 constexpr int kB = kAttnBlock;
-constexpr int kThreads = 320;
-constexpr int kMmaWarp = 8, kLoadWarp = 9;
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9;  // 10 and 11 only fill up the warpgroup
+// Registers a thread: 384 x 168 at launch, then 256 x 200 + 128 x 104 of them.
+constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr uint32_t kChunkBytes = kB * 128;  // 128 rows x 64 elements, 128-byte swizzle
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.44269504f;
@@ -117,18 +119,6 @@ __device__ __forceinline__ void ld32_dep(float* r) {
                  :
                  : "memory");
 }
-__device__ __forceinline__ void st32(uint32_t taddr, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
-      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
-}
-
 // V block as the B operand [keys (K)][dims (N)]: N-major, 128-byte swizzle.
 // 64 dims are one 128-byte row of the tile; the next 64 lie a chunk further
 // (leading offset), the next 8 keys 1024 bytes further (stride offset).
@@ -343,10 +333,6 @@ struct Ring {
 };
 
 // ------------------------------------------------------------------ softmax
-// One block of one row: scores in s (raw on entry), weights out as packed
-// pairs in pk, the row's maximum (log2 units) and sum updated.  Returns the
-// factor that O has to be scaled by (1: none).
-template <typename T, bool CAP, bool BIAS>
 struct RowState {
   float m = -INFINITY, l = 0.f;
   int lo = 0, hi = 0, pos = 0;
@@ -355,73 +341,125 @@ struct RowState {
 };
 
 struct ScoreConst {
-  float sc2;       // scale * log2(e); with a cap: scale / cap
-  float cap2;      // cap * log2(e)
-  float c0, c1, c2, c3;  // cap2 * tanh(u) = u (c0 + c1 u^2 + c2 u^4 + c3 u^6) for |u| <= 1/2
+  float sc2;             // scale * log2(e); with a cap: scale / cap
+  float cap2;            // cap * log2(e)
+  float c0, c1, c2, c3;  // cap2 tanh(sc2 s) = s (c0 + c1 s^2 + c2 s^4 + c3 s^6) for |sc2 s| <= 1/2
+  int forward;           // causal without prefix: no visible key lies behind its row
 };
 
-// cap2 tanh(u) for any u: 1 - 2 / (1 + e^(2u)).
-__device__ __forceinline__ float cap_any(float u, const ScoreConst& c) {
-  return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(u * (2.0f * kLog2e))), 1.0f);
+__device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
+
+// cap2 tanh(sc2 s) for any s: 1 - 2 / (1 + e^(2u)).
+__device__ __forceinline__ float cap_any(float s, const ScoreConst& c) {
+  return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(s * (c.sc2 * (2.0f * kLog2e)))), 1.0f);
+}
+// c0 + c1 z + c2 z^2 + c3 z^3 with z = s^2, for a pair.
+__device__ __forceinline__ float2 cap_poly(float2 s, const ScoreConst& c) {
+  const float2 z = __fmul2_rn(s, s);
+  float2 q = __ffma2_rn(both(c.c3), z, both(c.c2));
+  q = __ffma2_rn(q, z, both(c.c1));
+  return __ffma2_rn(q, z, both(c.c0));
 }
 
-// cap2 tanh(sc2 s) of 32 scores in place.  Near zero (|u| <= 1/2, all 32 of
-// every row of the warp) a polynomial on the FMA pipe; its absolute error is
-// 1.5e-7 of the cap.  The exponential form takes two steps of the 16-per-clock
-// pipe that the softmax already fills.
-__device__ __forceinline__ void cap32(float* s, const ScoreConst& c) {
-  float big = 0.f;
+// Column e of a block that begins at key0 is visible.
+struct Mask {
+  uint32_t w[4];
+  __device__ __forceinline__ Mask(int key0, int lo, int hi) {
 #pragma unroll
-  for (int e = 0; e < 32; e += 2) big = fmaxf(big, fmaxf(fabsf(s[e]), fabsf(s[e + 1])));
-  if (__all_sync(0xFFFFFFFFu, big * c.sc2 <= 0.5f)) {
-#pragma unroll
-    for (int e = 0; e < 32; e += 2) {
-      const float2 u = __fmul2_rn(make_float2(s[e], s[e + 1]), make_float2(c.sc2, c.sc2));
-      const float2 z = __fmul2_rn(u, u);
-      float2 q = __ffma2_rn(make_float2(c.c3, c.c3), z, make_float2(c.c2, c.c2));
-      q = __ffma2_rn(q, z, make_float2(c.c1, c.c1));
-      q = __ffma2_rn(q, z, make_float2(c.c0, c.c0));
-      q = __fmul2_rn(q, u);
-      s[e] = q.x;
-      s[e + 1] = q.y;
+    for (int i = 0; i < 4; ++i) {
+      // Visible columns [a, b) of this word.
+      const int a = min(max(lo - key0 - 32 * i, 0), 32), b = min(max(hi - key0 - 32 * i, 0), 32);
+      const uint32_t upto = b == 32 ? 0xFFFFFFFFu : (1u << b) - 1u;
+      w[i] = a < b ? upto & (0xFFFFFFFFu << a) : 0u;
     }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 32; ++e) s[e] = cap_any(s[e] * c.sc2, c);
   }
-}
+  __device__ __forceinline__ bool operator[](int e) const { return (w[e >> 5] >> (e & 31)) & 1u; }
+};
 
+// One block of one row: raw scores in s; the weights go to tensor memory at
+// `tp` as packed pairs, the row's maximum (log2 units) and sum are brought up
+// to date.  Returns the factor that O has to be scaled by (1: none).
+//
+// With a cap and no bias the transform is monotone, so the maximum is taken
+// over raw scores and the transform, the subtraction of the maximum and the
+// exponential are one sweep: 5.5 instructions a score, against 8 clocks of the
+// exponential pipe for a warp's 32.
+// The cap's polynomial serves a block whose scores all lie within half the cap
+// (error 1.5e-7 of the cap); the exponential form would take two more steps of
+// the pipe that the softmax already fills.
 template <typename T, bool CAP, bool BIAS>
-__device__ __forceinline__ float softmax_block(float* s, uint32_t* pk, RowState<T, CAP, BIAS>& r, const ScoreConst& c,
-                                               int key0, bool masked, bool first) {
+__device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& r, const ScoreConst& c, int key0,
+                                               bool masked, bool first) {
+  const Mask vis(key0, r.lo, r.hi);
+  bool near = true;  // every score of the warp within half the cap
   if constexpr (CAP) {
+    float mn[4], mx[4];
 #pragma unroll
-    for (int e = 0; e < kB; e += 32) cap32(s + e, c);
+    for (int i = 0; i < 4; ++i) mn[i] = mx[i] = s[i];
+#pragma unroll
+    for (int e = 4; e < kB; e += 8)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float y = e + 4 + i < kB ? s[e + 4 + i] : s[e + i];
+        mn[i] = fminf(fminf(mn[i], s[e + i]), y);
+        mx[i] = fmaxf(fmaxf(mx[i], s[e + i]), y);
+      }
+    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+    const float low = fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3]));
+    near = __all_sync(0xFFFFFFFFu, fmaxf(fabsf(top), fabsf(low)) * c.sc2 <= 0.5f);
+    if constexpr (BIAS) {
+      if (near) {
+#pragma unroll
+        for (int e = 0; e < kB; e += 2) {
+          const float2 x = make_float2(s[e], s[e + 1]), y = __fmul2_rn(cap_poly(x, c), x);
+          s[e] = y.x;
+          s[e + 1] = y.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kB; ++e) s[e] = cap_any(s[e], c);
+      }
+    }
   }
   if constexpr (BIAS) {
     const float d0 = static_cast<float>(key0 - r.pos);
+    // slope * (key - pos) where no visible key of the warp's rows lies behind
+    // its row, else -slope * |key - pos|.
+    const bool linear = c.forward || __all_sync(0xFFFFFFFFu, key0 + kB - 1 <= r.pos || !r.valid);
+    const float2 mul = both(CAP ? 1.0f : c.sc2);
+    if (linear) {
+      const float2 at0 = both(d0 * r.slope);
 #pragma unroll
-    for (int e = 0; e < kB; ++e) {
-      const float x = CAP ? s[e] : s[e] * c.sc2;
-      s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), x);
+      for (int e = 0; e < kB; e += 2) {
+        const float2 x = __ffma2_rn(make_float2(s[e], s[e + 1]), mul, at0);
+        const float2 y = __ffma2_rn(both(r.slope), make_float2(static_cast<float>(e), static_cast<float>(e + 1)), x);
+        s[e] = y.x;
+        s[e + 1] = y.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kB; ++e) s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), s[e] * mul.x);
     }
   }
   if (masked) {
-    const uint32_t n = static_cast<uint32_t>(r.hi - r.lo);
-    const uint32_t k = static_cast<uint32_t>(key0 - r.lo);
 #pragma unroll
-    for (int e = 0; e < kB; ++e) s[e] = k + e < n ? s[e] : -INFINITY;
+    for (int e = 0; e < kB; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
   }
   float mx[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mx[i] = fmaxf(s[2 * i], s[2 * i + 1]);
+  for (int i = 0; i < 4; ++i) mx[i] = fmaxf(s[i], s[i + 4]);
 #pragma unroll
   for (int e = 8; e < kB; e += 8)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(mx[i], fmaxf(s[e + 2 * i], s[e + 2 * i + 1]));
+    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(fmaxf(mx[i], s[e + i]), s[e + 4 + i]);
   float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-  constexpr bool kScaled = CAP || BIAS;  // s is in log2 units already
-  if constexpr (!kScaled) m *= c.sc2;
+  if constexpr (!BIAS) {
+    if constexpr (CAP) {
+      if (m > -INFINITY) m = cap_any(m, c);
+    } else {
+      m *= c.sc2;
+    }
+  }
   float factor = 1.0f;
   if (first) {
     r.m = m;
@@ -430,20 +468,40 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t* pk, RowState<
     r.l *= factor;
     r.m = m;
   }
-  const float base = r.m == -INFINITY ? 0.f : -r.m;
-  float2 sum[4];
+  const float2 base = both(r.m == -INFINITY ? 0.f : -r.m);
+  float2 sum[2] = {both(0.f), both(0.f)};
+  auto sweep = [&](auto transform) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) sum[i] = make_float2(0.f, 0.f);
-  const float2 mul = make_float2(kScaled ? 1.0f : c.sc2, kScaled ? 1.0f : c.sc2), add = make_float2(base, base);
+    for (int e0 = 0; e0 < kB; e0 += 32) {
+      uint32_t pk[16];
 #pragma unroll
-  for (int e = 0; e < kB; e += 2) {
-    const float2 x = make_float2(s[e], s[e + 1]);
-    const float2 y = kScaled ? __fadd2_rn(x, add) : __ffma2_rn(x, mul, add);
-    const float2 w = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
-    sum[(e >> 1) & 3] = __fadd2_rn(sum[(e >> 1) & 3], w);
-    pk[e >> 1] = pack2<T>(w.x, w.y);
+      for (int e = 0; e < 32; e += 2) {
+        const float2 y = transform(make_float2(s[e0 + e], s[e0 + e + 1]), e0 + e);
+        const float2 w = make_float2(ex2_ftz(y.x), ex2_ftz(y.y));
+        sum[(e >> 1) & 1] = __fadd2_rn(sum[(e >> 1) & 1], w);
+        pk[e >> 1] = pack2<T>(w.x, w.y);
+      }
+      tc_st_32x32b_x16(tp + e0 / 2, pk);
+    }
+  };
+  if constexpr (BIAS) {
+    sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
+  } else if constexpr (CAP) {
+    if (masked) {
+      sweep([&](float2 x, int e) {
+        const float2 y = near ? __ffma2_rn(cap_poly(x, c), x, base)
+                              : make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y);
+        return make_float2(vis[e] ? y.x : -INFINITY, vis[e + 1] ? y.y : -INFINITY);
+      });
+    } else if (near) {
+      sweep([&](float2 x, int) { return __ffma2_rn(cap_poly(x, c), x, base); });
+    } else {
+      sweep([&](float2 x, int) { return make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y); });
+    }
+  } else {
+    sweep([&](float2 x, int) { return __ffma2_rn(x, both(c.sc2), base); });
   }
-  const float2 a = __fadd2_rn(__fadd2_rn(sum[0], sum[1]), __fadd2_rn(sum[2], sum[3]));
+  const float2 a = __fadd2_rn(sum[0], sum[1]);
   r.l += a.x + a.y;
   return factor;
 }
@@ -511,6 +569,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     more = pc.qt * p.np < clamp_len(a.q_len, pc.b, a.Sq);
   }
 
+  if (warp >= kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------- loads
     Ring rg;
@@ -718,8 +778,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (!mbar_wait(&C.drain, 0, &dummy, p.wait_ns)) raise_error(p.err, abort_flag, kErrDrain);
     }
     __syncwarp();
+  }
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2;
     const int row = (warp & 3) * 32 + lane;
     const uint32_t lane_addr = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -728,15 +790,17 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (CAP) {
       c.sc2 = a.scale / a.cap;
       c.cap2 = a.cap * kLog2e;
-      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 1/2.
-      c.c0 = c.cap2 * 0.99999768f;
-      c.c1 = c.cap2 * -0.33320656f;
-      c.c2 = c.cap2 * 0.13145146f;
-      c.c3 = c.cap2 * -0.043372475f;
+      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 1/2, for s = u / sc2.
+      const float k2 = c.sc2 * c.sc2;
+      c.c0 = c.cap2 * c.sc2 * 0.99999768f;
+      c.c1 = c.cap2 * c.sc2 * k2 * -0.33320656f;
+      c.c2 = c.cap2 * c.sc2 * k2 * k2 * 0.13145146f;
+      c.c3 = c.cap2 * c.sc2 * k2 * k2 * k2 * -0.043372475f;
     } else {
       c.sc2 = a.scale * kLog2e;
       c.cap2 = c.c0 = c.c1 = c.c2 = c.c3 = 0.f;
     }
+    c.forward = a.causal && !a.prefix;
     uint32_t s_phase = 0, o_phase = 0;
     int piece = 0;
     bool ok = true;
@@ -753,7 +817,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int qt = pc.qt + (SPLIT ? 0 : t);
       const int i = qt * p.np + static_cast<int>(p.fd_gp.div(row)), h = pc.hg * p.gp + row - static_cast<int>(p.fd_gp.div(row)) * p.gp;
       const int q_len = clamp_len(a.q_len, pc.b, a.Sq), k_len = clamp_len(a.k_len, pc.b, a.Sk);
-      RowState<T, CAP, BIAS> st;
+      RowState st;
       st.valid = row < fill && i < q_len;
       int wlo = 0, whi = 0x7FFFFFFF;
       if (st.valid) {
@@ -775,16 +839,13 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (live) {
           tc_fence_after();
           float s[kB];
-          uint32_t pk[kB / 2];
 #pragma unroll
           for (int e = 0; e < kB; e += 32) ld32(my_s + e, s + e);
           tc_wait_ld();
 #pragma unroll
           for (int e = 0; e < kB; e += 32) ld32_dep(s + e);
           const bool masked = j * kB < wlo || (j + 1) * kB > whi;
-          const float f = softmax_block<T, CAP, BIAS>(s, pk, st, c, j * kB, masked, done == 0);
-          st32(my_s, pk);
-          st32(my_s + 32, pk + 32);
+          const float f = softmax_block<T, CAP, BIAS>(s, my_s, st, c, j * kB, masked, done == 0);
           if (__any_sync(0xFFFFFFFFu, f != 1.0f)) {
             // The product of the block before is complete: these scores were
             // issued after it.
