@@ -135,6 +135,42 @@ __device__ __forceinline__ uint32_t idesc_f32(int N, bool bn) {
          (static_cast<uint32_t>(kB >> 4) << 24);
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+// Largest (smallest) of the 128 scores.
+__device__ __forceinline__ float max128(const float* s) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = max3(s[i], s[i + 4], s[i + 8]);
+#pragma unroll
+  for (int e = 12; e + 8 <= kB; e += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[e + i], s[e + 4 + i]);
+  m[0] = max3(m[0], s[kB - 4], s[kB - 3]);
+  m[1] = max3(m[1], s[kB - 2], s[kB - 1]);
+  return fmaxf(max3(m[0], m[1], m[2]), m[3]);
+}
+__device__ __forceinline__ float min128(const float* s) {
+  float m[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) m[i] = min3(s[i], s[i + 4], s[i + 8]);
+#pragma unroll
+  for (int e = 12; e + 8 <= kB; e += 8)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) m[i] = min3(m[i], s[e + i], s[e + 4 + i]);
+  m[0] = min3(m[0], s[kB - 4], s[kB - 3]);
+  m[1] = min3(m[1], s[kB - 2], s[kB - 1]);
+  return fminf(min3(m[0], m[1], m[2]), m[3]);
+}
+
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
 template <>
@@ -392,21 +428,11 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
                                                bool masked, bool first) {
   const Mask vis(key0, r.lo, r.hi);
   bool near = true;  // every score of the warp within half the cap
+  float m;
   if constexpr (CAP) {
-    float mn[4], mx[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mn[i] = mx[i] = s[i];
-#pragma unroll
-    for (int e = 4; e < kB; e += 8)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float y = e + 4 + i < kB ? s[e + 4 + i] : s[e + i];
-        mn[i] = fminf(fminf(mn[i], s[e + i]), y);
-        mx[i] = fmaxf(fmaxf(mx[i], s[e + i]), y);
-      }
-    const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-    const float low = fminf(fminf(mn[0], mn[1]), fminf(mn[2], mn[3]));
-    near = __all_sync(0xFFFFFFFFu, fmaxf(fabsf(top), fabsf(low)) * c.sc2 <= 0.5f);
+    m = max128(s);
+    const float low = min128(s);
+    near = __all_sync(0xFFFFFFFFu, fmaxf(fabsf(m), fabsf(low)) * c.sc2 <= 0.5f);
     if constexpr (BIAS) {
       if (near) {
 #pragma unroll
@@ -445,14 +471,7 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
 #pragma unroll
     for (int e = 0; e < kB; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
   }
-  float mx[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) mx[i] = fmaxf(s[i], s[i + 4]);
-#pragma unroll
-  for (int e = 8; e < kB; e += 8)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx[i] = fmaxf(fmaxf(mx[i], s[e + i]), s[e + 4 + i]);
-  float m = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+  if (!CAP || BIAS || masked) m = max128(s);
   if constexpr (!BIAS) {
     if constexpr (CAP) {
       if (m > -INFINITY) m = cap_any(m, c);
@@ -645,9 +664,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       tc_fence_after();
       if (lane == 0) {
         const uint32_t qa = smem_u32(sq) + (SPLIT ? 0 : t) * kBlockBytes, kb = smem_u32(ring) + slot * kBlockBytes;
-        for (int k = 0; k < ksteps; ++k) {
-          const uint32_t o = (k >> 2) * kChunkBytes + (k & 3) * 32;
-          mma_ss(ts[t], sw128_kmajor_desc(qa + o), sw128_kmajor_desc(kb + o), id_s, k > 0);
+        const uint64_t qd = sw128_kmajor_desc(qa), kd = sw128_kmajor_desc(kb);
+#pragma unroll
+        for (int k = 0; k < HDP / 16; ++k) {
+          constexpr uint32_t kc = kChunkBytes >> 4;
+          const uint32_t o = (k >> 2) * kc + (k & 3) * 2;  // 16-byte units
+          if (k < ksteps) mma_ss(ts[t], qd + o, kd + o, id_s, k > 0);
         }
         tc_commit(&C.s_full[t]);
       }
@@ -656,10 +678,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     auto values = [&](int t, int slot, bool first, bool last) {
       tc_fence_after();
       if (lane == 0) {
-        const uint32_t vb = smem_u32(ring) + slot * kBlockBytes;
+        const uint64_t vd = v_desc(smem_u32(ring) + slot * kBlockBytes);
 #pragma unroll
-        for (int k = 0; k < kB / 16; ++k)
-          mma_ts(to[t], ts[t] + 8 * k, v_desc(vb + 2048 * k), id_o, !first || k > 0);
+        for (int k = 0; k < kB / 16; ++k) mma_ts(to[t], ts[t] + 8 * k, vd + 128 * k, id_o, !first || k > 0);
         if (last) tc_commit(&C.o_full[t]);
       }
       __syncwarp();
