@@ -85,6 +85,19 @@ struct Ctl {
 static_assert(sizeof(Ctl) + 1024 <= kCtlBytes, "control block plus alignment");
 
 // ------------------------------------------------------------- PTX pieces
+// A value that all lanes share, marked as such: what is computed from it can
+// stay in uniform registers, where the UMMA's operands have to be.
+__device__ __forceinline__ int uni(int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
+// True in one lane of a converged warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t p;
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "elect.sync _|q, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(p));
+  return p != 0;
+}
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t acc) {
   tc_mma_bf16(d, ad, bd, idesc, acc);  // kind::f16; the types are in idesc
 }
@@ -350,6 +363,13 @@ __device__ __forceinline__ Blocks block_range(const AttnPlan& p, const Piece& s)
     if (r.j0[0] == r.j1[0]) r.j0[0] = r.j1[0] = r.j0[1];  // an empty tile takes no part in the union
     if (r.j0[1] == r.j1[1]) r.j0[1] = r.j1[1] = r.j0[0];
   }
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    r.j0[t] = uni(r.j0[t]);
+    r.j1[t] = uni(r.j1[t]);
+  }
+  r.lo = uni(r.lo);
+  r.hi = uni(r.hi);
   return r;
 }
 
@@ -537,7 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* sq = base;
   uint8_t* ring = base + q_bytes<HDP, SPLIT>();
   Ctl& C = *reinterpret_cast<Ctl*>(ring + NST * kBlockBytes);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
   volatile int* abort_flag = &C.abort;
   const yb_attn_args& a = p.a;
 
@@ -566,7 +586,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tm = C.tmem;
+  const uint32_t tm = uni(C.tmem);
   const uint32_t ts[2] = {tm, tm + kB}, to[2] = {tm + 2 * kB, tm + 2 * kB + HDP};
 
   // Pieces of this CTA: split mode walks its share; row mode has one pair of
@@ -662,9 +682,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto scores = [&](int t, int slot) {
       tc_fence_after();
-      if (lane == 0) {
-        const uint32_t qa = smem_u32(sq) + (SPLIT ? 0 : t) * kBlockBytes, kb = smem_u32(ring) + slot * kBlockBytes;
-        const uint64_t qd = sw128_kmajor_desc(qa), kd = sw128_kmajor_desc(kb);
+      const uint64_t qd = sw128_kmajor_desc(smem_u32(sq) + (SPLIT ? 0 : t) * kBlockBytes);
+      const uint64_t kd = sw128_kmajor_desc(smem_u32(ring) + slot * kBlockBytes);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < HDP / 16; ++k) {
           constexpr uint32_t kc = kChunkBytes >> 4;
@@ -673,21 +693,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_commit(&C.s_full[t]);
       }
-      __syncwarp();
     };
     auto values = [&](int t, int slot, bool first, bool last) {
       tc_fence_after();
-      if (lane == 0) {
-        const uint64_t vd = v_desc(smem_u32(ring) + slot * kBlockBytes);
+      const uint64_t vd = v_desc(smem_u32(ring) + slot * kBlockBytes);
+      if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < kB / 16; ++k) mma_ts(to[t], ts[t] + 8 * k, vd + 128 * k, id_o, !first || k > 0);
         if (last) tc_commit(&C.o_full[t]);
       }
-      __syncwarp();
     };
     auto release = [&](int slot) {
-      if (lane == 0) tc_commit(&C.kv_empty[slot]);
-      __syncwarp();
+      if (elect_one()) tc_commit(&C.kv_empty[slot]);
     };
     // Zeroes the value rows of block j that no row sees.
     auto clean = [&](int slot, int j, const Blocks& r) {
@@ -764,23 +781,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (again) rg.next<NST>();
             if (!wait(&C.kv_full[v.slot], v.phase, kErrWaitFull)) break;
             clean(v.slot, j, r);
+            if (again && !wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
+#pragma unroll
             for (int t = 0; t < 2; ++t) {
               if (j >= r.j0[t] && j < r.j1[t]) {
                 if (!wait(&C.p_full[t], p_phase[t], kErrWaitAccFull)) break;
                 p_phase[t] ^= 1u;
                 values(t, v.slot, j == r.j0[t], j + 1 == r.j1[t]);
               }
-              if (again && j + 1 >= r.j0[t] && j + 1 < r.j1[t]) {
-                if (!wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
-                scores(t, k.slot);
-              }
+              if (again && j + 1 >= r.j0[t] && j + 1 < r.j1[t]) scores(t, k.slot);
             }
             if (!ok) break;
             release(v.slot);
-            if (again) {
-              if (!wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
-              release(k.slot);
-            }
+            if (again) release(k.slot);
           }
         }
       }
@@ -792,7 +805,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         more = false;
     }
     // Everything issued has to finish before tensor memory goes.
-    if (lane == 0) {
+    if (elect_one()) {
       int dummy = 0;
       if (q_open) mbar_wait(&C.q_full, q_phase, &dummy, p.wait_ns);
       tc_commit(&C.drain);
