@@ -86,6 +86,16 @@ def test_ragged():
             run_case(5, Sq, Sk, 4, 2, 64, causal=causal, q_len=i32(ql), k_len=i32(kl))
 
 
+def test_tiles_without_keys_between_others():
+    """Many short sequences, every second one without a key: a CTA goes through tiles with and without work."""
+    B = 400
+    kl = [(b * 37) % 500 + 1 if b % 2 else 0 for b in range(B)]
+    ql = [3 if b % 5 else 0 for b in range(B)]
+    for causal in (False, True):
+        run_case(B, 3, 512, 8, 4, 64, causal=causal, q_len=i32(ql), k_len=i32(kl))
+        run_case(60, 3, 3000, 8, 4, 64, causal=causal, k_len=i32([6 * k for k in kl[:60]]))
+
+
 def test_prefix():
     for Sq, Sk in [(300, 300), (100, 700), (1, 400)]:
         run_case(4, Sq, Sk, 4, 2, 64, causal=True, prefix=i32([0, 1, 200, 10 ** 6]))

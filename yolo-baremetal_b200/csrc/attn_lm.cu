@@ -796,6 +796,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (again) release(k.slot);
           }
         }
+      } else if (SPLIT && piece > 0) {
+        // Once a piece also where there is nothing to do: a wait two phases
+        // behind would pass on the parity of an earlier one.
+        wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty);
       }
       if (!ok) break;
       ++piece;
