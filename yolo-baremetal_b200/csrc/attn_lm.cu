@@ -11,9 +11,11 @@
 //
 // CTA (10 warps): warps 0-3 and 4-7 are two softmax pipelines, warp 8 issues
 // the UMMAs, warp 9 the TMA loads into a ring of 128-key blocks of K and V.
-// Tensor memory: S0, S1 (128 columns each; P overwrites the first half of its
-// S as packed 16-bit pairs and is read back as the A operand), O0, O1.  While
-// one pipeline does its exponentials the tensor cores work for the other.
+// Tensor memory: two S buffers of 64 columns a pipeline (half a key block each;
+// P overwrites the first half of its S as packed 16-bit pairs and is read back
+// as the A operand), O0, O1.  While the softmax works on one buffer the tensor
+// cores fill the other; with one buffer of 128 columns a pipeline waited 1,400
+// clocks of 3,900 a block at D = 128 for its product and next scores.
 //   row mode    the pipelines own two row tiles and share each K and V block;
 //   split mode  the pipelines take the even and odd blocks of one row tile, and
 //               the blocks of all tiles are dealt out evenly to a grid of one
@@ -22,8 +24,8 @@
 //               between CTAs leaves (max, sum, O) in scratch, and
 //               attn_join_kernel joins the pieces in their order.
 //
-// The running maximum is only raised when it grows by more than 2^8 (then O is
-// rescaled in place): until then weights up to 256 are as exact, and O stays
+// The running maximum is only raised when weights outgrow their range (then O
+// is rescaled in place): until then larger weights are as exact, and O stays
 // untouched in tensor memory.  The maximum in use never enters the result.
 //
 // A weight of zero times an infinite or NaN value would be NaN, so value rows
@@ -50,6 +52,7 @@ namespace yb {
 namespace {
 
 constexpr int kB = kAttnBlock;
+constexpr int kH = kB / 2;  // keys of a half block: one S buffer
 constexpr int kThreads = 384;
 constexpr int kMmaWarp = 8, kLoadWarp = 9;  // 10 and 11 only fill up the warpgroup
 // Registers a thread: 384 x 168 at launch, then 256 x 200 + 128 x 104 of them.
@@ -58,6 +61,10 @@ constexpr uint32_t kChunkBytes = kB * 128;  // 128 rows x 64 elements, 128-byte 
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.44269504f;
 constexpr float kRaise = 8.0f;  // log2 growth of the maximum that O is rescaled for
+// Sum of a block up to which the maximum at hand serves it: fp16 weights end at
+// 65504, bf16 ones and fp32 sums near 2^127, which leaves 2^31 for keys and values.
+template <typename T>
+constexpr float kFits = std::is_same<T, __half>::value ? 4096.0f : 7.9228163e28f;
 constexpr int kSmemMax = 232448;
 constexpr int kCtlBytes = 3072;  // control block, after up to 1 KB of alignment
 
@@ -76,7 +83,7 @@ __host__ __device__ constexpr int smem_bytes() {
 }
 
 struct Ctl {
-  uint64_t q_full, s_full[2], p_full[2], o_full[2], o_empty, ml_full, drain;
+  uint64_t q_full, s_full[2][2], p_full[2][2], o_full[2][2], o_empty, ml_full, drain;
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
   int abort;
@@ -158,29 +165,29 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
 }
-// Largest (smallest) of the 128 scores.
-__device__ __forceinline__ float max128(const float* s) {
+// Largest (smallest) of a half block's scores; NaN is passed over.
+__device__ __forceinline__ float max_of(const float* s) {
   float m[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = max3(s[i], s[i + 4], s[i + 8]);
 #pragma unroll
-  for (int e = 12; e + 8 <= kB; e += 8)
+  for (int e = 12; e + 8 <= kH; e += 8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = max3(m[i], s[e + i], s[e + 4 + i]);
-  m[0] = max3(m[0], s[kB - 4], s[kB - 3]);
-  m[1] = max3(m[1], s[kB - 2], s[kB - 1]);
+  m[0] = max3(m[0], s[kH - 4], s[kH - 3]);
+  m[1] = max3(m[1], s[kH - 2], s[kH - 1]);
   return fmaxf(max3(m[0], m[1], m[2]), m[3]);
 }
-__device__ __forceinline__ float min128(const float* s) {
+__device__ __forceinline__ float min_of(const float* s) {
   float m[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) m[i] = min3(s[i], s[i + 4], s[i + 8]);
 #pragma unroll
-  for (int e = 12; e + 8 <= kB; e += 8)
+  for (int e = 12; e + 8 <= kH; e += 8)
 #pragma unroll
     for (int i = 0; i < 4; ++i) m[i] = min3(m[i], s[e + i], s[e + 4 + i]);
-  m[0] = min3(m[0], s[kB - 4], s[kB - 3]);
-  m[1] = min3(m[1], s[kB - 2], s[kB - 1]);
+  m[0] = min3(m[0], s[kH - 4], s[kH - 3]);
+  m[1] = min3(m[1], s[kH - 2], s[kH - 1]);
   return fminf(min3(m[0], m[1], m[2]), m[3]);
 }
 
@@ -397,10 +404,11 @@ struct RowState {
 };
 
 struct ScoreConst {
-  float sc2;             // scale * log2(e); with a cap: scale / cap
-  float cap2;            // cap * log2(e)
-  float c0, c1, c2, c3;  // cap2 tanh(sc2 s) = s (c0 + c1 s^2 + c2 s^4 + c3 s^6) for |sc2 s| <= 1/2
-  int forward;           // causal without prefix: no visible key lies behind its row
+  float sc2;         // scale * log2(e); with a cap: scale / cap
+  float cap2;        // cap * log2(e)
+  float c0, c1, c2;  // cap2 tanh(sc2 s) = s (c0 + c1 s^2 + c2 s^4) for |s| <= near
+  float near, near2;
+  bool forward;  // causal without prefix: no visible key lies behind its row
 };
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
@@ -409,20 +417,18 @@ __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 __device__ __forceinline__ float cap_any(float s, const ScoreConst& c) {
   return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(s * (c.sc2 * (2.0f * kLog2e)))), 1.0f);
 }
-// c0 + c1 z + c2 z^2 + c3 z^3 with z = s^2, for a pair.
-__device__ __forceinline__ float2 cap_poly(float2 s, const ScoreConst& c) {
-  const float2 z = __fmul2_rn(s, s);
-  float2 q = __ffma2_rn(both(c.c3), z, both(c.c2));
-  q = __ffma2_rn(q, z, both(c.c1));
+// c0 + c1 z + c2 z^2 with z = s^2, for a pair.
+__device__ __forceinline__ float2 cap_poly(float2 z, const ScoreConst& c) {
+  const float2 q = __ffma2_rn(both(c.c2), z, both(c.c1));
   return __ffma2_rn(q, z, both(c.c0));
 }
 
-// Column e of a block that begins at key0 is visible.
+// Column e of a half block that begins at key0 is visible.
 struct Mask {
-  uint32_t w[4];
+  uint32_t w[2];
   __device__ __forceinline__ Mask(int key0, int lo, int hi) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       // Visible columns [a, b) of this word.
       const int a = min(max(lo - key0 - 32 * i, 0), 32), b = min(max(hi - key0 - 32 * i, 0), 32);
       const uint32_t upto = b == 32 ? 0xFFFFFFFFu : (1u << b) - 1u;
@@ -432,86 +438,27 @@ struct Mask {
   __device__ __forceinline__ bool operator[](int e) const { return (w[e >> 5] >> (e & 31)) & 1u; }
 };
 
-// One block of one row: raw scores in s; the weights go to tensor memory at
+// One half block of one row: raw scores in s; the weights go to tensor memory at
 // `tp` as packed pairs, the row's maximum (log2 units) and sum are brought up
 // to date.  Returns the factor that O has to be scaled by (1: none).
 //
-// With a cap and no bias the transform is monotone, so the maximum is taken
-// over raw scores and the transform, the subtraction of the maximum and the
-// exponential are one sweep: 5.5 instructions a score, against 8 clocks of the
-// exponential pipe for a warp's 32.
-// The cap's polynomial serves a block whose scores all lie within half the cap
-// (error 1.5e-7 of the cap); the exponential form would take two more steps of
-// the pipe that the softmax already fills.
+// The maximum in use only has to keep weights in range, so a half block that every
+// row of the warp sees whole is tried with the one at hand, in one sweep
+// without a search for its own: its sum, taken anyway, tells whether a weight
+// left the range.  Only then, in the first block and where masks cut is the
+// maximum searched.
+//
+// cap tanh(s / cap) is a polynomial on the FMA pipe while all scores lie within
+// 3/8 of the cap (error 8e-7 of the cap), else 1 - 2 / (1 + e^2u), with two
+// more steps of the exponential pipe that bounds the sweep.
 template <typename T, bool CAP, bool BIAS>
 __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& r, const ScoreConst& c, int key0,
                                                bool masked, bool first) {
-  const Mask vis(key0, r.lo, r.hi);
-  bool near = true;  // every score of the warp within half the cap
-  float m;
-  if constexpr (CAP) {
-    m = max128(s);
-    const float low = min128(s);
-    near = __all_sync(0xFFFFFFFFu, fmaxf(fabsf(m), fabsf(low)) * c.sc2 <= 0.5f);
-    if constexpr (BIAS) {
-      if (near) {
-#pragma unroll
-        for (int e = 0; e < kB; e += 2) {
-          const float2 x = make_float2(s[e], s[e + 1]), y = __fmul2_rn(cap_poly(x, c), x);
-          s[e] = y.x;
-          s[e + 1] = y.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kB; ++e) s[e] = cap_any(s[e], c);
-      }
-    }
-  }
-  if constexpr (BIAS) {
-    const float d0 = static_cast<float>(key0 - r.pos);
-    // slope * (key - pos) where no visible key of the warp's rows lies behind
-    // its row, else -slope * |key - pos|.
-    const bool linear = c.forward || __all_sync(0xFFFFFFFFu, key0 + kB - 1 <= r.pos || !r.valid);
-    const float2 mul = both(CAP ? 1.0f : c.sc2);
-    if (linear) {
-      const float2 at0 = both(d0 * r.slope);
-#pragma unroll
-      for (int e = 0; e < kB; e += 2) {
-        const float2 x = __ffma2_rn(make_float2(s[e], s[e + 1]), mul, at0);
-        const float2 y = __ffma2_rn(both(r.slope), make_float2(static_cast<float>(e), static_cast<float>(e + 1)), x);
-        s[e] = y.x;
-        s[e + 1] = y.y;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < kB; ++e) s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), s[e] * mul.x);
-    }
-  }
-  if (masked) {
-#pragma unroll
-    for (int e = 0; e < kB; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
-  }
-  if (!CAP || BIAS || masked) m = max128(s);
-  if constexpr (!BIAS) {
-    if constexpr (CAP) {
-      if (m > -INFINITY) m = cap_any(m, c);
-    } else {
-      m *= c.sc2;
-    }
-  }
-  float factor = 1.0f;
-  if (first) {
-    r.m = m;
-  } else if (m > r.m + kRaise) {
-    factor = ex2_ftz(r.m - m);
-    r.l *= factor;
-    r.m = m;
-  }
-  const float2 base = both(r.m == -INFINITY ? 0.f : -r.m);
-  float2 sum[2] = {both(0.f), both(0.f)};
+  float2 sum[2];
   auto sweep = [&](auto transform) {
+    sum[0] = sum[1] = both(0.f);
 #pragma unroll
-    for (int e0 = 0; e0 < kB; e0 += 32) {
+    for (int e0 = 0; e0 < kH; e0 += 32) {
       uint32_t pk[16];
 #pragma unroll
       for (int e = 0; e < 32; e += 2) {
@@ -522,26 +469,104 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
       }
       tc_st_32x32b_x16(tp + e0 / 2, pk);
     }
+    const float2 a = __fadd2_rn(sum[0], sum[1]);
+    return a.x + a.y;
   };
-  if constexpr (BIAS) {
-    sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
-  } else if constexpr (CAP) {
-    if (masked) {
-      sweep([&](float2 x, int e) {
-        const float2 y = near ? __ffma2_rn(cap_poly(x, c), x, base)
-                              : make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y);
-        return make_float2(vis[e] ? y.x : -INFINITY, vis[e + 1] ? y.y : -INFINITY);
-      });
-    } else if (near) {
-      sweep([&](float2 x, int) { return __ffma2_rn(cap_poly(x, c), x, base); });
-    } else {
-      sweep([&](float2 x, int) { return make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y); });
+  const float d0 = static_cast<float>(key0 - r.pos);
+  // The bias is slope * (key - pos) where no visible key of the warp's rows
+  // lies behind its row, else -slope * |key - pos|.
+  const bool linear = BIAS && (c.forward || __all_sync(0xFFFFFFFFu, key0 + kH - 1 <= r.pos || !r.valid));
+  bool fits = true;  // the maximum at hand served this row
+  if (!masked && !first && (!BIAS || linear) && __all_sync(0xFFFFFFFFu, r.m > -INFINITY || !r.valid)) {
+    const float2 add = both(BIAS ? fmaf(d0, r.slope, -r.m) : -r.m);
+    float far[2] = {0.f, 0.f};
+    const float t = sweep([&](float2 x, int e) {
+      const float2 at = BIAS ? __ffma2_rn(both(r.slope), make_float2(static_cast<float>(e), static_cast<float>(e + 1)), add)
+                             : add;
+      if constexpr (CAP) {
+        const float2 z = __fmul2_rn(x, x);
+        far[(e >> 1) & 1] = max3(far[(e >> 1) & 1], z.x, z.y);
+        return __ffma2_rn(cap_poly(z, c), x, at);
+      } else {
+        return __ffma2_rn(x, both(c.sc2), at);
+      }
+    });
+    fits = t <= kFits<T>;
+    if constexpr (CAP) {
+      fits = fits && fmaxf(far[0], far[1]) <= c.near2;
     }
-  } else {
-    sweep([&](float2 x, int) { return __ffma2_rn(x, both(c.sc2), base); });
+    fits = fits || !r.valid;
+    if (__all_sync(0xFFFFFFFFu, fits)) {
+      r.l += t;
+      return 1.0f;
+    }
   }
-  const float2 a = __fadd2_rn(sum[0], sum[1]);
-  r.l += a.x + a.y;
+
+  const Mask vis(key0, r.lo, r.hi);
+  bool near = true;  // every visible score of the warp's rows within half the cap
+  if constexpr (CAP) {
+    if (masked) {  // NaN takes no part in minima and maxima
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : __uint_as_float(0x7FC00000u);
+    }
+    const float far = fmaxf(fabsf(max_of(s)), fabsf(min_of(s)));
+    near = __all_sync(0xFFFFFFFFu, !(far > c.near) || !r.valid);
+  }
+  if constexpr (BIAS) {
+    if constexpr (CAP) {
+      if (near) {
+#pragma unroll
+        for (int e = 0; e < kH; e += 2) {
+          const float2 x = make_float2(s[e], s[e + 1]), y = __fmul2_rn(cap_poly(__fmul2_rn(x, x), c), x);
+          s[e] = y.x;
+          s[e + 1] = y.y;
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kH; ++e) s[e] = cap_any(s[e], c);
+      }
+    }
+    const float mul = CAP ? 1.0f : c.sc2;
+    if (linear) {
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = fmaf(r.slope, d0 + static_cast<float>(e), s[e] * mul);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), s[e] * mul);
+    }
+  }
+  if (masked && (!CAP || BIAS)) {
+#pragma unroll
+    for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
+  }
+  float m = fmaxf(max_of(s), -INFINITY);
+  if constexpr (!BIAS) {
+    if constexpr (CAP) {
+      if (m > -INFINITY) m = cap_any(m, c);
+    } else {
+      m *= c.sc2;
+    }
+  }
+  float factor = 1.0f;
+  if (first) {
+    r.m = m;
+  } else if (m > r.m + (fits ? kRaise : 0.f)) {
+    factor = ex2_ftz(r.m - m);
+    r.l *= factor;
+    r.m = m;
+  }
+  const float2 base = both(r.m == -INFINITY ? 0.f : -r.m);
+  if constexpr (BIAS) {
+    r.l += sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
+  } else if constexpr (CAP) {
+    r.l += sweep([&](float2 x, int e) {
+      const float2 y = near ? __ffma2_rn(cap_poly(__fmul2_rn(x, x), c), x, base)
+                            : make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y);
+      return masked ? make_float2(vis[e] ? y.x : -INFINITY, vis[e + 1] ? y.y : -INFINITY) : y;
+    });
+  } else {
+    r.l += sweep([&](float2 x, int) { return __ffma2_rn(x, both(c.sc2), base); });
+  }
   return factor;
 }
 
@@ -565,9 +590,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     mbar_init(&C.q_full, 1);
     for (int t = 0; t < 2; ++t) {
-      mbar_init(&C.s_full[t], 1);
-      mbar_init(&C.p_full[t], 4);
-      mbar_init(&C.o_full[t], 1);
+      for (int h = 0; h < 2; ++h) {
+        mbar_init(&C.s_full[t][h], 1);
+        mbar_init(&C.p_full[t][h], 4);
+        mbar_init(&C.o_full[t][h], 1);
+      }
     }
     mbar_init(&C.o_empty, 4);
     mbar_init(&C.ml_full, 4);
@@ -634,16 +661,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           ++loads;
           rg.next<NST>();
         };
-        if constexpr (SPLIT) {
-          for (int j = j0; j <= j1 && ok && j1 > j0; ++j) {
-            if (j < j1) load(&tmk, p.k_bmul, j);
-            if (j > j0 && ok) load(&tmv, p.v_bmul, j - 1);
-          }
-        } else {
-          for (int j = j0; j < j1 && ok; ++j) {
-            load(&tmk, p.k_bmul, j);
-            if (ok) load(&tmv, p.v_bmul, j);
-          }
+        // Ring order: K then V of one block after another; in split mode of
+        // pairs of blocks, one for each pipeline.
+        constexpr int kSet = SPLIT ? 2 : 1;
+        for (int j = j0; j < j1 && ok; j += kSet) {
+          for (int x = j; x < min(j + kSet, j1) && ok; ++x) load(&tmk, p.k_bmul, x);
+          for (int x = j; x < min(j + kSet, j1) && ok; ++x) load(&tmv, p.v_bmul, x);
         }
       }
       ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
@@ -667,10 +690,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else if (warp == kMmaWarp) {
     // -------------------------------------------------------------- UMMAs
     Ring rg;
-    uint32_t p_phase[2] = {0, 0}, q_phase = 0;
+    uint32_t p_phase[2] = {0, 0}, q_phase = 0;  // of a pipeline, both halves
     int piece = 0;
     bool ok = true, q_open = false;
-    const uint32_t id_s = idesc_f32<T>(kB, false), id_o = idesc_f32<T>(16 * ksteps, true);
+    const uint32_t id_s = idesc_f32<T>(kH, false), id_o = idesc_f32<T>(16 * ksteps, true);
     const uint32_t q_tx = static_cast<uint32_t>(NCH * 128 * fill);
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       // The lanes agree, so that none is left behind at a warp barrier.
@@ -680,27 +703,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       return ok;
     };
-    auto scores = [&](int t, int slot) {
+    // Scores of half h of the block in `slot` into the pipeline's buffer h, and
+    // the product of the weights there with the values of that half.
+    auto scores = [&](int t, int h, int slot) {
       tc_fence_after();
       const uint64_t qd = sw128_kmajor_desc(smem_u32(sq) + (SPLIT ? 0 : t) * kBlockBytes);
-      const uint64_t kd = sw128_kmajor_desc(smem_u32(ring) + slot * kBlockBytes);
+      const uint64_t kd = sw128_kmajor_desc(smem_u32(ring) + slot * kBlockBytes + h * (kH * 128));
       if (elect_one()) {
 #pragma unroll
         for (int k = 0; k < HDP / 16; ++k) {
           constexpr uint32_t kc = kChunkBytes >> 4;
           const uint32_t o = (k >> 2) * kc + (k & 3) * 2;  // 16-byte units
-          if (k < ksteps) mma_ss(ts[t], qd + o, kd + o, id_s, k > 0);
+          if (k < ksteps) mma_ss(ts[t] + h * kH, qd + o, kd + o, id_s, k > 0);
         }
-        tc_commit(&C.s_full[t]);
+        tc_commit(&C.s_full[t][h]);
       }
     };
-    auto values = [&](int t, int slot, bool first, bool last) {
+    auto values = [&](int t, int h, int slot, bool first) {
       tc_fence_after();
-      const uint64_t vd = v_desc(smem_u32(ring) + slot * kBlockBytes);
+      const uint64_t vd = v_desc(smem_u32(ring) + slot * kBlockBytes + h * (kH * 128));
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < kB / 16; ++k) mma_ts(to[t], ts[t] + 8 * k, vd + 128 * k, id_o, !first || k > 0);
-        if (last) tc_commit(&C.o_full[t]);
+        for (int k = 0; k < kH / 16; ++k)
+          mma_ts(to[t], ts[t] + h * kH + 8 * k, vd + 128 * k, id_o, !first || h > 0 || k > 0);
+        tc_commit(&C.o_full[t][h]);
       }
     };
     auto release = [&](int slot) {
@@ -738,63 +764,56 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!wait(&C.q_full, q_phase, kErrWaitFull)) break;
         q_open = false;
         q_phase ^= 1u;
-        if constexpr (SPLIT) {
-          const int n = j1 - j0;
-          int vslot = 0;
-          uint32_t vphase = 0;
-          for (int i = 0; i < n + 2 && ok; ++i) {
-            // Ring order: K0, K1, V0, K2, V1, ...  V of block i - 2 comes
-            // after K of block i - 1.
-            if (i >= 2) {
-              const int v = i - 2, t = v & 1;
-              if (!wait(&C.kv_full[vslot], vphase, kErrWaitFull)) break;
-              clean(vslot, j0 + v, r);
-              if (v == 0 && piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
-              if (!wait(&C.p_full[t], p_phase[t], kErrWaitAccFull)) break;
-              p_phase[t] ^= 1u;
-              values(t, vslot, v < 2, v + 2 >= n);
-              release(vslot);
-            }
-            if (i < n) {
-              if (!wait(&C.kv_full[rg.slot], rg.phase, kErrWaitFull)) break;
-              scores(i & 1, rg.slot);
-              release(rg.slot);
-              rg.next<NST>();
-            }
-            if (i >= 1 && i <= n) {  // the ring's next block is V of block i - 1
-              vslot = rg.slot;
-              vphase = rg.phase;
-              rg.next<NST>();
-            }
-          }
-        } else {
-          if (!wait(&C.kv_full[rg.slot], rg.phase, kErrWaitFull)) break;
-          for (int t = 0; t < 2; ++t)
-            if (j0 >= r.j0[t] && j0 < r.j1[t]) scores(t, rg.slot);
-          release(rg.slot);
-          rg.next<NST>();
-          for (int j = j0; j < j1 && ok; ++j) {
-            const Ring v = rg;
+        // Step by step: one block, which both pipelines share, or in split
+        // mode a pair of blocks, one for each.  The scores of a step's halves
+        // go out when the weights of the step before them are used up, so the
+        // softmax finds its next half ready.
+        constexpr int kSet = SPLIT ? 2 : 1;
+        const int steps = (j1 - j0 + kSet - 1) / kSet;
+        auto takes = [&](int t, int n) {  // pipeline t has a block in step n
+          return SPLIT ? n < steps && 2 * n + t < j1 - j0 : n < steps && j0 + n >= r.j0[t] && j0 + n < r.j1[t];
+        };
+        int ks[2] = {0, 0}, vs[2] = {0, 0};
+        auto take = [&](int n, int (&slot)[2]) {  // waits for the blocks of step n next in the ring
+          for (int x = 0; x < kSet && kSet * n + x < j1 - j0; ++x) {
+            if (!wait(&C.kv_full[rg.slot], rg.phase, kErrWaitFull)) return false;
+            slot[x] = rg.slot;
             rg.next<NST>();
-            const Ring k = rg;
-            const bool again = j + 1 < j1;
-            if (again) rg.next<NST>();
-            if (!wait(&C.kv_full[v.slot], v.phase, kErrWaitFull)) break;
-            clean(v.slot, j, r);
-            if (again && !wait(&C.kv_full[k.slot], k.phase, kErrWaitFull)) break;
+          }
+          return true;
+        };
+        auto drop = [&](int n, const int (&slot)[2]) {
+          for (int x = 0; x < kSet && kSet * n + x < j1 - j0; ++x) release(slot[x]);
+        };
+        if (!take(0, ks)) break;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+          if (takes(t, 0)) {
+            scores(t, 0, ks[SPLIT ? t : 0]);
+            scores(t, 1, ks[SPLIT ? t : 0]);
+          }
+        drop(0, ks);
+        // The earlier piece's O has been read.
+        if (SPLIT && piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
+        for (int n = 0; n < steps && ok; ++n) {
+          if (!take(n, vs)) break;
+          for (int x = 0; x < kSet && kSet * n + x < j1 - j0; ++x) clean(vs[x], j0 + kSet * n + x, r);
+          if (n + 1 < steps && !take(n + 1, ks)) break;
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-              if (j >= r.j0[t] && j < r.j1[t]) {
-                if (!wait(&C.p_full[t], p_phase[t], kErrWaitAccFull)) break;
-                p_phase[t] ^= 1u;
-                values(t, v.slot, j == r.j0[t], j + 1 == r.j1[t]);
+              if (takes(t, n)) {
+                if (!wait(&C.p_full[t][h], p_phase[t], kErrWaitAccFull)) break;
+                values(t, h, vs[SPLIT ? t : 0], n == 0 || !takes(t, n - 1));
               }
-              if (again && j + 1 >= r.j0[t] && j + 1 < r.j1[t]) scores(t, k.slot);
+              if (takes(t, n + 1)) scores(t, h, ks[SPLIT ? t : 0]);
             }
-            if (!ok) break;
-            release(v.slot);
-            if (again) release(k.slot);
-          }
+          if (!ok) break;
+          for (int t = 0; t < 2; ++t)
+            if (takes(t, n)) p_phase[t] ^= 1u;
+          drop(n, vs);
+          if (n + 1 < steps) drop(n + 1, ks);
         }
       } else if (SPLIT && piece > 0) {
         // Once a piece also where there is nothing to do: a wait two phases
@@ -828,18 +847,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (CAP) {
       c.sc2 = a.scale / a.cap;
       c.cap2 = a.cap * kLog2e;
-      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 1/2, for s = u / sc2.
+      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 3/8,
+      // for s = u / sc2; no polynomial where its coefficients could leave fp32.
       const float k2 = c.sc2 * c.sc2;
-      c.c0 = c.cap2 * c.sc2 * 0.99999768f;
-      c.c1 = c.cap2 * c.sc2 * k2 * -0.33320656f;
-      c.c2 = c.cap2 * c.sc2 * k2 * k2 * 0.13145146f;
-      c.c3 = c.cap2 * c.sc2 * k2 * k2 * k2 * -0.043372475f;
+      c.c0 = c.cap2 * c.sc2 * 0.9999854f;
+      c.c1 = c.cap2 * c.sc2 * k2 * -0.33248851f;
+      c.c2 = c.cap2 * c.sc2 * k2 * k2 * 0.12098849f;
+      c.near = c.sc2 >= 1.0f / 4096.0f && c.sc2 <= 4096.0f ? 0.375f / c.sc2 : -1.0f;
+      c.near2 = c.near > 0.f ? c.near * c.near : -1.0f;
     } else {
       c.sc2 = a.scale * kLog2e;
-      c.cap2 = c.c0 = c.c1 = c.c2 = c.c3 = 0.f;
+      c.cap2 = c.c0 = c.c1 = c.c2 = c.near = c.near2 = 0.f;
     }
     c.forward = a.causal && !a.prefix;
-    uint32_t s_phase = 0, o_phase = 0;
+    uint32_t s_phase = 0;
     int piece = 0;
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
@@ -870,43 +891,52 @@ __global__ void __launch_bounds__(kThreads, 1)
       whi = __reduce_min_sync(0xFFFFFFFFu, whi);
       const int step = SPLIT ? 2 : 1;
       const int jb = r.j0[t] + (SPLIT ? t : 0);
-      int done = 0;
-      for (int j = jb; j < r.j1[t]; j += step, ++done) {
-        if (!wait(&C.s_full[t], s_phase, kErrWaitAccFull)) break;
-        s_phase ^= 1u;
-        if (live) {
-          tc_fence_after();
-          float s[kB];
+      int done = 0;  // half blocks
+      for (int j = jb; j < r.j1[t] && ok; j += step) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h, ++done) {
+          if (!wait(&C.s_full[t][h], s_phase, kErrWaitAccFull)) break;
+          if (live) {
+            tc_fence_after();
+            const uint32_t buf = my_s + h * kH;
+            const int key0 = j * kB + h * kH;
+            float s[kH];
 #pragma unroll
-          for (int e = 0; e < kB; e += 32) ld32(my_s + e, s + e);
-          tc_wait_ld();
+            for (int e = 0; e < kH; e += 32) ld32(buf + e, s + e);
+            tc_wait_ld();
 #pragma unroll
-          for (int e = 0; e < kB; e += 32) ld32_dep(s + e);
-          const bool masked = j * kB < wlo || (j + 1) * kB > whi;
-          const float f = softmax_block<T, CAP, BIAS>(s, my_s, st, c, j * kB, masked, done == 0);
-          if (__any_sync(0xFFFFFFFFu, f != 1.0f)) {
-            // The product of the block before is complete: these scores were
-            // issued after it.
-            for (int e = 0; e < 16 * ksteps; e += 16) {
-              uint32_t o[16];
-              tc_ld_32x32b_x16(to[t] + lane_addr + e, o);
-              tc_wait_ld();
-              tc_ld_dep(o);
+            for (int e = 0; e < kH; e += 32) ld32_dep(s + e);
+            const bool masked = key0 < wlo || key0 + kH > whi;
+            const float f = softmax_block<T, CAP, BIAS>(s, buf, st, c, key0, masked, done == 0);
+            if (__any_sync(0xFFFFFFFFu, f != 1.0f)) {
+              // After the product before this one: of this block's first half,
+              // or of the second half of the block before.  (s_phase is the
+              // block's parity; the product before that one was complete when
+              // these scores were, so the barrier is never two phases off.)
+              if (!wait(&C.o_full[t][h ^ 1], h ? s_phase : s_phase ^ 1u, kErrWaitAccFull)) break;
+              tc_fence_after();
+              for (int e = 0; e < 16 * ksteps; e += 16) {
+                uint32_t o[16];
+                tc_ld_32x32b_x16(to[t] + lane_addr + e, o);
+                tc_wait_ld();
+                tc_ld_dep(o);
 #pragma unroll
-              for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
-              tc_st_32x32b_x16(to[t] + lane_addr + e, o);
+                for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(__uint_as_float(o[x]) * f);
+                tc_st_32x32b_x16(to[t] + lane_addr + e, o);
+              }
             }
+            tc_wait_st();
+            tc_fence_before();
           }
-          tc_wait_st();
-          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&C.p_full[t][h]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&C.p_full[t]);
+        s_phase ^= 1u;
       }
       if (!ok) break;
-      if (done) {
-        if (!wait(&C.o_full[t], o_phase, kErrWaitAccFull)) break;
-        o_phase ^= 1u;
+      if (done) {  // the last block's products
+        if (!wait(&C.o_full[t][0], s_phase ^ 1u, kErrWaitAccFull)) break;
+        if (!wait(&C.o_full[t][1], s_phase ^ 1u, kErrWaitAccFull)) break;
       }
       float w[2] = {1.f, 0.f}, m = st.m, l = st.l;
       bool have[2] = {done > 0, false};
