@@ -98,6 +98,7 @@ static_assert(sizeof(Ctl) + 1024 <= kCtlBytes, "control block plus alignment");
 // A value that all lanes share, marked as such: what is computed from it can
 // stay in uniform registers, where the UMMA's operands have to be.
 __device__ __forceinline__ int uni(int x) { return __shfl_sync(0xFFFFFFFFu, x, 0); }
+__device__ __forceinline__ void prefetch_l1(const void* p) { asm volatile("prefetch.global.L1 [%0];" ::"l"(p)); }
 // True in one lane of a converged warp.
 __device__ __forceinline__ bool elect_one() {
   uint32_t p;
@@ -327,11 +328,20 @@ __device__ __forceinline__ Keys tile_keys(const AttnPlan& p, int b, int qt) {
     return k;
   }
   int lo = 0x7FFFFFFF, hi = 0;
-  for (int i = i0 + static_cast<int>(threadIdx.x & 31); i < i1; i += 32) {
-    const RowSpan s = row_span(p.a, b, i, q_len, k_len);
-    if (s.lo < s.hi) {
-      lo = min(lo, s.lo);
-      hi = max(hi, s.hi);
+  const int prefix = p.a.causal && p.a.prefix ? min(p.a.prefix[b], k_len) : 0;
+  const int2* range = reinterpret_cast<const int2*>(p.a.key_range) + static_cast<long long>(b) * p.a.Sq;
+  int2 own[kB / 32];  // all rows' loads in flight together
+#pragma unroll
+  for (int x = 0; x < kB / 32; ++x) own[x] = range[min(i0 + 32 * x + static_cast<int>(threadIdx.x & 31), i1 - 1)];
+#pragma unroll
+  for (int x = 0; x < kB / 32; ++x) {
+    const int i = min(i0 + 32 * x + static_cast<int>(threadIdx.x & 31), i1 - 1);
+    int end = k_len;  // as row_span
+    if (p.a.causal) end = max(min(k_len, k_len - q_len + i + 1), prefix);
+    const int first = max(0, own[x].x), last = min(end, own[x].y);
+    if (first < last) {
+      lo = min(lo, first);
+      hi = max(hi, last);
     }
   }
   lo = __reduce_min_sync(0xFFFFFFFFu, lo);
@@ -446,10 +456,11 @@ struct Mask {
 // to date.  Returns the factor that O has to be scaled by (1: none).
 //
 // The maximum in use only has to keep weights in range, so a half block that every
-// row of the warp sees whole is tried with the one at hand, in one sweep
+// row of the warp sees whole (or whose hidden scores are -infinity beforehand,
+// where no cap follows) is tried with the one at hand, in one sweep
 // without a search for its own: its sum, taken anyway, tells whether a weight
-// left the range.  Only then, in the first block and where masks cut is the
-// maximum searched.
+// left the range.  Only then and in a row's first half block is the maximum
+// searched.
 //
 // cap tanh(s / cap) is a polynomial on the FMA pipe while all scores lie within
 // 3/8 of the cap (error 8e-7 of the cap), else 1 - 2 / (1 + e^2u), with two
@@ -480,7 +491,12 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   // lies behind its row, else -slope * |key - pos|.
   const bool linear = BIAS && (c.forward || __all_sync(0xFFFFFFFFu, key0 + kH - 1 <= r.pos || !r.valid));
   bool fits = true;  // the maximum at hand served this row
-  if (!masked && !first && (!BIAS || linear) && __all_sync(0xFFFFFFFFu, r.m > -INFINITY || !r.valid)) {
+  if (!(CAP && masked) && !first && (!BIAS || linear) && __all_sync(0xFFFFFFFFu, r.m > -INFINITY || !r.valid)) {
+    if (!CAP && masked) {
+      const Mask vis(key0, r.lo, r.hi);
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
+    }
     const float2 add = both(BIAS ? fmaf(d0, r.slope, -r.m) : -r.m);
     float far[2] = {0.f, 0.f};
     const float t = sweep([&](float2 x, int e) {
@@ -589,6 +605,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* abort_flag = &C.abort;
   const yb_attn_args& a = p.a;
 
+  Piece pc;
+  if constexpr (!SPLIT) {
+    // Row mode has one pair of tiles, the last rows (the most keys of a causal
+    // prompt) first.  What its roles are about to read is on its way while
+    // barriers and tensor memory are set up.
+    const int bh = a.B * p.groups, pairs = (p.tiles + 1) / 2;
+    const int x = blockIdx.x / bh, y = blockIdx.x - x * bh;
+    pc.b = y / p.groups;
+    pc.hg = y - pc.b * p.groups;
+    pc.qt = 2 * (pairs - 1 - x);
+    if (threadIdx.x < 32) {
+      if (a.q_len) prefetch_l1(a.q_len + pc.b);
+      if (a.k_len) prefetch_l1(a.k_len + pc.b);
+      if (a.prefix) prefetch_l1(a.prefix + pc.b);
+    }
+    const int i = pc.qt * p.np + static_cast<int>(threadIdx.x);
+    if (a.key_range && static_cast<int>(threadIdx.x) < 2 * p.np && i < a.Sq)
+      prefetch_l1(a.key_range + 2 * (static_cast<long long>(pc.b) * a.Sq + i));
+  }
   pdl_trigger();  // the join's blocks may come up meanwhile; they wait for this grid's end
   if (threadIdx.x == 0) {
     mbar_init(&C.q_full, 1);
@@ -608,6 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     C.abort = 0;
     mbar_fence_init();
+    prefetch_tmap(&tmq);
+    prefetch_tmap(&tmk);
+    prefetch_tmap(&tmv);
   }
   if (warp == kMmaWarp) {
     tmem_alloc(&C.tmem, kTmemCols);
@@ -619,10 +657,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tm = uni(C.tmem);
   const uint32_t ts[2] = {tm, tm + kB}, to[2] = {tm + 2 * kB, tm + 2 * kB + HDP};
 
-  // Pieces of this CTA: split mode walks its share; row mode has one pair of
-  // tiles, the last rows (the most keys of a causal prompt) first.
+  // Pieces of this CTA: split mode walks its share, row mode has its pair.
   Walk walk;
-  Piece pc;
   const int ksteps = (a.D + 15) / 16;
   const int fill = p.gp * p.np;  // rows of a full tile
   bool more;
@@ -630,11 +666,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     walk.seek(p, blockIdx.x, gridDim.x);
     more = walk.next(p, &pc);
   } else {
-    const int bh = a.B * p.groups, pairs = (p.tiles + 1) / 2;
-    const int x = blockIdx.x / bh, y = blockIdx.x - x * bh;
-    pc.b = y / p.groups;
-    pc.hg = y - pc.b * p.groups;
-    pc.qt = 2 * (pairs - 1 - x);
     more = pc.qt * p.np < clamp_len(a.q_len, pc.b, a.Sq);
   }
 
