@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int n = 0; n < steps && ok; ++n) {
           if (!take(n, vs)) break;
           for (int x = 0; x < kSet && kSet * n + x < j1 - j0; ++x) clean(vs[x], j1 - 1 - kSet * n - x, r);
-          if (n + 1 < steps && !take(n + 1, ks)) break;
+          if (!SPLIT && n + 1 < steps && !take(n + 1, ks)) break;
 #pragma unroll
           for (int h = 1; h >= 0; --h)
 #pragma unroll
@@ -840,14 +840,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               if (takes(t, n)) {
                 if (!wait(&C.p_full[t][h], p_phase[t], kErrWaitAccFull)) break;
                 values(t, h, vs[SPLIT ? t : 0], n == 0 || !takes(t, n - 1));
+                if (SPLIT && h == 0) release(vs[t]);
               }
-              if (takes(t, n + 1)) scores(t, h, ks[SPLIT ? t : 0]);
+              // Split mode is bound by memory: the next keys may come while the
+              // first product of the step runs, and slots go back one by one.
+              if (SPLIT && h == 1 && t == 0 && n + 1 < steps && !take(n + 1, ks)) break;
+              if (takes(t, n + 1)) {
+                scores(t, h, ks[SPLIT ? t : 0]);
+                if (SPLIT && h == 0) release(ks[t]);
+              }
             }
           if (!ok) break;
           for (int t = 0; t < 2; ++t)
             if (takes(t, n)) p_phase[t] ^= 1u;
-          drop(n, vs);
-          if (n + 1 < steps) drop(n + 1, ks);
+          if (!SPLIT) {
+            drop(n, vs);
+            if (n + 1 < steps) drop(n + 1, ks);
+          }
         }
       } else if (SPLIT && piece > 0) {
         // Once a piece also where there is nothing to do: a wait two phases
