@@ -26,138 +26,224 @@ struct alignas(sizeof(T) * VEC) Chunk {
   T v[VEC];
 };
 
-template <typename T, int VEC, int NS>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const yb_qk_args a, int group_log, int tokens) {
-  __shared__ float2 turn[kMaxTokens * (kMaxD / 2)];  // cos, sin of each token's pairs
+// VEC floats of shared memory (16-byte aligned where VEC is 4 or 8).
+template <int VEC>
+__device__ __forceinline__ void shared_words(const float* p, float* v) {
+  if constexpr (VEC % 4 == 0) {
+#pragma unroll
+    for (int e = 0; e < VEC; e += 4) {
+      const float4 x = *reinterpret_cast<const float4*>(p + e);
+      v[e] = x.x, v[e + 1] = x.y, v[e + 2] = x.z, v[e + 3] = x.w;
+    }
+  } else {
+    v[0] = *p;
+  }
+}
+
+// A token of the CTA: where its first head rows of q, k and v come from and go
+// to (null: not in use, or outside the cache), and its position.
+struct Token {
+  const void* src[3];
+  void* dst[3];
+  long long pos;
+  int live;
+};
+
+template <typename T, int VEC, int NS, bool INTER>
+__global__ void __launch_bounds__(kThreads, NS == 1 ? 4 : 3)
+    qk_norm_rope_kernel(const __grid_constant__ yb_qk_args a, int group_log, int tokens) {
+  // cos and sin of each token's pairs, and both weights: read as whole 16-byte
+  // words.
+  __shared__ __align__(16) float turn_c[kMaxTokens * (kMaxD / 2)], turn_s[kMaxTokens * (kMaxD / 2)];
+  __shared__ __align__(16) float weights[2][kMaxD];
+  __shared__ Token token[kMaxTokens];
   const int half = a.R / 2;
+  const int pitch = (half + 3) & ~3;  // of a token's angles
   const long long total = static_cast<long long>(a.B) * a.S;
   const long long first = static_cast<long long>(blockIdx.x) * tokens;
-  for (int i = threadIdx.x; i < tokens * half; i += kThreads) {
-    const int k = i / half, f = i - k * half;
-    if (first + k >= total) break;
-    const int b = static_cast<int>((first + k) / a.S), t = static_cast<int>(first + k - static_cast<long long>(b) * a.S);
-    const long long pos =
-        a.positions ? a.positions[first + k] : (a.start ? static_cast<long long>(a.start[b]) : 0ll) + t;
-    const double turns = static_cast<double>(pos) * a.inv_freq[f] * 0.15915494309189533577;  // 1 / (2 pi)
+  if (threadIdx.x < static_cast<unsigned>(tokens)) {
+    const long long x = first + threadIdx.x;
+    Token k{};
+    if (x < total) {
+      const int b = static_cast<int>(x / a.S), t = static_cast<int>(x - static_cast<long long>(b) * a.S);
+      const int length = a.length ? a.length[b] : a.S, start = a.start ? a.start[b] : 0;
+      const int at = a.positions ? a.positions[x] : 0;  // three loads in flight
+      k.live = t < length;
+      const long long row = static_cast<long long>(start) + t;
+      k.pos = a.positions ? static_cast<long long>(at) : row;
+      if (k.live) {
+        auto from = [&](const void* p, const long long* st) {
+          return static_cast<const void*>(static_cast<const T*>(p) + b * st[0] + t * st[1]);
+        };
+        auto to = [&](void* p, const long long* st, long long r) {
+          return static_cast<void*>(static_cast<T*>(p) + b * st[0] + r * st[1]);
+        };
+        if (a.q) {
+          k.src[0] = from(a.q, a.q_stride);
+          k.dst[0] = to(a.q_out, a.q_out_stride, t);
+        }
+        if (row >= 0 && row < a.cache_rows) {
+          if (a.k) {
+            k.src[1] = from(a.k, a.k_stride);
+            k.dst[1] = to(a.k_out, a.k_out_stride, row);
+          }
+          if (a.v) {
+            k.src[2] = from(a.v, a.v_stride);
+            k.dst[2] = to(a.v_out, a.v_out_stride, row);
+          }
+        }
+      }
+    }
+    token[threadIdx.x] = k;
+  }
+  for (int d = threadIdx.x; d < a.D; d += kThreads) {
+    weights[0][d] = (a.q_weight ? a.q_weight[d] : 1.0f) + a.weight_add;
+    weights[1][d] = (a.k_weight ? a.k_weight[d] : 1.0f) + a.weight_add;
+  }
+  __syncthreads();
+
+  // This lane's chunks of any row: offsets, and first pair (-1: not rotated).
+  const int group = 1 << group_log, lane = threadIdx.x & (group - 1);
+  const int slots = a.D / 2 / VEC;
+  int o0[NS], o1[NS], f0[NS];
+#pragma unroll
+  for (int s = 0; s < NS; ++s) {
+    const int slot = s * group + lane;
+    f0[s] = -1;
+    if (INTER) {
+      o0[s] = 2 * slot * VEC;
+      o1[s] = o0[s] + VEC;
+      if (o0[s] < a.R) f0[s] = slot * VEC;
+    } else if (slot * VEC < half) {
+      o0[s] = slot * VEC;
+      o1[s] = half + slot * VEC;
+      f0[s] = slot * VEC;
+    } else {
+      o0[s] = a.R + slot * VEC - half;
+      o1[s] = o0[s] + (a.D - a.R) / 2;
+    }
+  }
+
+  // Rows (head rows of q, k and v of the CTA's tokens) go round the groups;
+  // the next one's loads are under way while one is worked on, the first one's
+  // while the angles are formed.
+  const int rows = a.Hq + a.Hkv * (a.v ? 2 : 1);
+  const int groups = kThreads >> group_log;
+  // Every lane of a warp makes the same number of rounds (the sums shuffle).
+  const int rounds = (tokens * rows + groups - 1) / groups;
+  int k = 0, head = threadIdx.x >> group_log;  // of the row to fetch next
+  struct Row {
+    Chunk<T, VEC> c0[NS], c1[NS];
+    T* dst;
+    int k, kind;
+    bool live;
+  };
+  auto fetch = [&](Row& r) {
+    while (head >= rows) head -= rows, ++k;
+    r.k = k;
+    r.kind = head < a.Hq ? 0 : head < a.Hq + a.Hkv ? 1 : 2;
+    const int h = head - (r.kind == 0 ? 0 : r.kind == 1 ? a.Hq : a.Hq + a.Hkv);
+    const T* src = k < tokens ? static_cast<const T*>(token[k].src[r.kind]) : nullptr;
+    r.live = src != nullptr;
+    if (r.live) {
+      src += h * (r.kind == 0 ? a.q_stride[2] : r.kind == 1 ? a.k_stride[2] : a.v_stride[2]);
+      r.dst = static_cast<T*>(token[k].dst[r.kind]) +
+              h * (r.kind == 0 ? a.q_out_stride[2] : r.kind == 1 ? a.k_out_stride[2] : a.v_out_stride[2]);
+#pragma unroll
+      for (int s = 0; s < NS; ++s)
+        if (s * group + lane < slots) {
+          r.c0[s] = *reinterpret_cast<const Chunk<T, VEC>*>(src + o0[s]);
+          r.c1[s] = *reinterpret_cast<const Chunk<T, VEC>*>(src + o1[s]);
+        }
+    }
+    head += groups;
+  };
+  Row cur, next;
+  fetch(cur);
+
+  // One token's angles after another, a quarter of the CTA on each of four.
+  const int quarter = kThreads / kMaxTokens;
+  for (int i = threadIdx.x; i < kMaxTokens * (tokens == 1 ? kThreads : quarter); i += kThreads) {
+    const int x = tokens == 1 ? 0 : i / quarter;
+    if (x >= tokens || !token[x].live) continue;
+    for (int f = tokens == 1 ? i : i - x * quarter; f < half; f += tokens == 1 ? kThreads : quarter) {
+    const double turns = static_cast<double>(token[x].pos) * a.inv_freq[f] * 0.15915494309189533577;  // 1 / (2 pi)
     const double r = turns - rint(turns);
     const float hi = static_cast<float>(r), lo = static_cast<float>(r - static_cast<double>(hi)) * 6.28318531f;
     float s, c;
     sincospif(2.0f * hi, &s, &c);
-    turn[i] = make_float2(c - s * lo, s + c * lo);
+    turn_c[x * pitch + f] = c - s * lo;
+    turn_s[x * pitch + f] = s + c * lo;
+    }
   }
   __syncthreads();
 
-  const int group = 1 << group_log, lane = threadIdx.x & (group - 1);
-  const int slots = a.D / 2 / VEC;
-  const int rows = a.Hq + a.Hkv * (a.v ? 2 : 1);
-  const int end = tokens * rows;
-  // Every lane of a warp makes the same number of rounds (the sums shuffle).
-  const int rounds = (end + (kThreads >> group_log) - 1) / (kThreads >> group_log);
+  const float inv_d = 1.0f / static_cast<float>(a.D);
   for (int n = 0; n < rounds; ++n) {
-    const int item = n * (kThreads >> group_log) + (threadIdx.x >> group_log);
-    const int k = item / rows, head = item - k * rows;
-    bool live = item < end && first + k < total;
-    int b = 0, t = 0;
-    if (live) {
-      b = static_cast<int>((first + k) / a.S);
-      t = static_cast<int>(first + k - static_cast<long long>(b) * a.S);
-      live = !a.length || t < a.length[b];
-    }
-    const int kind = head < a.Hq ? 0 : head < a.Hq + a.Hkv ? 1 : 2;
-    const T* src = nullptr;
-    T* dst = nullptr;
-    if (live) {
-      const int h = kind == 0 ? head : kind == 1 ? head - a.Hq : head - a.Hq - a.Hkv;
-      const void* in = kind == 0 ? a.q : kind == 1 ? a.k : a.v;
-      void* out = kind == 0 ? a.q_out : kind == 1 ? a.k_out : a.v_out;
-      const long long* si = kind == 0 ? a.q_stride : kind == 1 ? a.k_stride : a.v_stride;
-      const long long* so = kind == 0 ? a.q_out_stride : kind == 1 ? a.k_out_stride : a.v_out_stride;
-      long long row = t;
-      if (kind) {
-        if (a.start) row += a.start[b];
-        live = row >= 0 && row < a.cache_rows;
-      }
-      src = static_cast<const T*>(in) + b * si[0] + t * si[1] + h * si[2];
-      dst = static_cast<T*>(out) + b * so[0] + row * so[1] + h * so[2];
-    }
-    Chunk<T, VEC> c0[NS], c1[NS];
-    int o0[NS], o1[NS], f0[NS];  // offsets of the two chunks, first pair (-1: not rotated)
-    float sum = 0.f;
+    if (n + 1 < rounds) fetch(next);
+    float2 squares = make_float2(0.f, 0.f);
+    if (cur.live && cur.kind < 2) {
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      const int slot = s * group + lane;
-      f0[s] = -1;
-      if (a.interleaved) {
-        o0[s] = 2 * slot * VEC;
-        o1[s] = o0[s] + VEC;
-        if (o0[s] < a.R) f0[s] = slot * VEC;
-      } else if (slot * VEC < half) {
-        o0[s] = slot * VEC;
-        o1[s] = half + slot * VEC;
-        f0[s] = slot * VEC;
-      } else {
-        o0[s] = a.R + slot * VEC - half;
-        o1[s] = o0[s] + (a.D - a.R) / 2;
-      }
-      if (live && slot < slots) {
-        c0[s] = *reinterpret_cast<const Chunk<T, VEC>*>(src + o0[s]);
-        c1[s] = *reinterpret_cast<const Chunk<T, VEC>*>(src + o1[s]);
-        if (kind < 2) {
+      for (int s = 0; s < NS; ++s)
+        if (s * group + lane < slots) {
 #pragma unroll
           for (int e = 0; e < VEC; ++e) {
-            const float x = to_f(c0[s].v[e]), y = to_f(c1[s].v[e]);
-            sum = fmaf(x, x, sum);
-            sum = fmaf(y, y, sum);
+            const float2 x = make_float2(to_f(cur.c0[s].v[e]), to_f(cur.c1[s].v[e]));
+            squares = __ffma2_rn(x, x, squares);
           }
         }
-      }
     }
+    float sum = squares.x + squares.y;
     for (int m = group >> 1; m; m >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, m);
-    if (!live) continue;
-    const float r = 1.0f / sqrtf(sum / static_cast<float>(a.D) + a.eps);
-    const float* w = kind == 0 ? a.q_weight : a.k_weight;
+    if (cur.live) {
+      const float r = rsqrtf(fmaf(sum, inv_d, a.eps));
+      const float* w = weights[cur.kind == 0 ? 0 : 1];
 #pragma unroll
-    for (int s = 0; s < NS; ++s) {
-      if (s * group + lane >= slots) continue;
-      if (kind < 2) {
-        float y[2 * VEC];
+      for (int s = 0; s < NS; ++s) {
+        if (s * group + lane >= slots) continue;
+        if (cur.kind < 2) {
+          // y[e] = (chunk 0's element e, chunk 1's element e).
+          float2 y[VEC];
+          float w0[VEC], w1[VEC];
+          shared_words<VEC>(w + o0[s], w0);
+          shared_words<VEC>(w + o1[s], w1);
+          const float2 r2 = make_float2(r, r);
 #pragma unroll
-        for (int e = 0; e < 2 * VEC; ++e) {
-          const int d = e < VEC ? o0[s] + e : o1[s] + e - VEC;
-          const float x = to_f(e < VEC ? c0[s].v[e] : c1[s].v[e - VEC]);
-          y[e] = x * r * ((w ? w[d] : 1.0f) + a.weight_add);
-        }
-        if (f0[s] >= 0) {
+          for (int e = 0; e < VEC; ++e)
+            y[e] = __fmul2_rn(__fmul2_rn(make_float2(to_f(cur.c0[s].v[e]), to_f(cur.c1[s].v[e])), r2),
+                              make_float2(w0[e], w1[e]));
+          if (f0[s] >= 0) {
+            float tc[VEC], ts[VEC];
+            shared_words<VEC>(turn_c + cur.k * pitch + f0[s], tc);
+            shared_words<VEC>(turn_s + cur.k * pitch + f0[s], ts);
+            if constexpr (!INTER) {
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) {
-            const float2 cs = turn[k * half + f0[s] + e];
-            float p, q;
-            if (a.interleaved) {
-              p = y[2 * e];
-              q = y[2 * e + 1];
+              for (int e = 0; e < VEC; ++e)  // (p c - q s, q c + p s)
+                y[e] = __ffma2_rn(make_float2(y[e].y, y[e].x), make_float2(-ts[e], ts[e]),
+                                  __fmul2_rn(y[e], make_float2(tc[e], tc[e])));
+            } else if constexpr (VEC == 1) {
+              y[0] = make_float2(y[0].x * tc[0] - y[0].y * ts[0], y[0].y * tc[0] + y[0].x * ts[0]);
             } else {
-              p = y[e];
-              q = y[e + VEC];
-            }
-            const float u = p * cs.x - q * cs.y, z = q * cs.x + p * cs.y;
-            if (a.interleaved) {
-              y[2 * e] = u;
-              y[2 * e + 1] = z;
-            } else {
-              y[e] = u;
-              y[e + VEC] = z;
+#pragma unroll
+              for (int e = 0; e < VEC; e += 2) {  // pairs e / 2 of chunk 0 and (VEC + e) / 2 of chunk 1
+                const float2 c2 = make_float2(tc[e / 2], tc[(VEC + e) / 2]), s2 = make_float2(ts[e / 2], ts[(VEC + e) / 2]);
+                const float2 p = y[e], q = y[e + 1];
+                y[e] = __ffma2_rn(q, make_float2(-s2.x, -s2.y), __fmul2_rn(p, c2));
+                y[e + 1] = __ffma2_rn(p, s2, __fmul2_rn(q, c2));
+              }
             }
           }
-        }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          c0[s].v[e] = from_f<T>(y[e]);
-          c1[s].v[e] = from_f<T>(y[e + VEC]);
+          for (int e = 0; e < VEC; ++e) {
+            cur.c0[s].v[e] = from_f<T>(y[e].x);
+            cur.c1[s].v[e] = from_f<T>(y[e].y);
+          }
         }
+        *reinterpret_cast<Chunk<T, VEC>*>(cur.dst + o0[s]) = cur.c0[s];
+        *reinterpret_cast<Chunk<T, VEC>*>(cur.dst + o1[s]) = cur.c1[s];
       }
-      *reinterpret_cast<Chunk<T, VEC>*>(dst + o0[s]) = c0[s];
-      *reinterpret_cast<Chunk<T, VEC>*>(dst + o1[s]) = c1[s];
     }
+    cur = next;
   }
 }
 
@@ -185,11 +271,15 @@ cudaError_t launch(const yb_qk_args& a, cudaStream_t s) {
   int group_log = 0;
   while (group_log < 5 && (1 << group_log) < slots) ++group_log;
   const long long total = static_cast<long long>(a.B) * a.S;
-  // A token per CTA spreads a decode step over the SMs; four share the
-  // launch and the angle stage once the grid is many waves deep.
-  const int tokens = total >= 4096 ? kMaxTokens : 1;
-  qk_norm_rope_kernel<T, VEC, NS>
-      <<<static_cast<unsigned>((total + tokens - 1) / tokens), kThreads, 0, s>>>(a, group_log, tokens);
+  // A token per CTA spreads a decode step over the SMs; four share what comes
+  // before their rows once there are CTAs enough for two on each SM (3,003
+  // fp32 tokens: 20.6 us one by one, 14.4 by fours).
+  const int tokens = total >= 2 * 148 * kMaxTokens ? kMaxTokens : 1;
+  const unsigned grid = static_cast<unsigned>((total + tokens - 1) / tokens);
+  if (a.interleaved)
+    qk_norm_rope_kernel<T, VEC, NS, true><<<grid, kThreads, 0, s>>>(a, group_log, tokens);
+  else
+    qk_norm_rope_kernel<T, VEC, NS, false><<<grid, kThreads, 0, s>>>(a, group_log, tokens);
   return cudaGetLastError();
 }
 
