@@ -16,12 +16,19 @@
 //     top-k, weights as well for top-p; it names the step that holds the
 //     border;
 //   3a at most kList tokens down to that step (the usual case): all go to CTA 0,
-//     which ranks them by comparing all pairs and finishes the row;
+//     which ranks them and finishes the row;
 //   3b else the step that holds the border is split further by composites
 //     (order-preserving key, ~index), which are all distinct, so ties need no
 //     rule of their own, until kList of them are left to rank; what stays
-//     above the cut is summed per warp and CTA, and the 32 runs of the CTA that
-//     holds the goal are scanned.
+//     above the cut is summed per warp and CTA, and the run of the warp that
+//     holds the goal is scanned.
+//
+// Measured: one row of 32,000 fp32 logits with top-k 50 and top-p 0.95 10.8 us
+// in the kernel, of which the cluster's four barriers and the exchange of the
+// histogram are about half: latency.  256 unfiltered rows of 131,072 fp32
+// logits 87 us (1.5 TB/s): about 45 instructions and 14 fp64 operations a
+// token, half of the issue slots; the rest are the barriers between the load,
+// the maximum and the sums, with three CTAs an SM to fill them.
 #include <cooperative_groups.h>
 
 #include <atomic>
