@@ -23,7 +23,8 @@ def attn_args(**kw):
 BAD_ATTN = [
     dict(B=-1), dict(Sq=-1), dict(Sk=-1), dict(Hq=0), dict(Hkv=0), dict(Hkv=3), dict(D=0), dict(D=4), dict(D=60),
     dict(D=136), dict(dtype=0), dict(dtype=3), dict(scale=0.0), dict(scale=-1.0), dict(scale=float("nan")),
-    dict(scale=float("inf")), dict(cap=-1.0), dict(cap=float("nan")), dict(causal=2), dict(prefix=64),
+    dict(scale=float("inf")), dict(scale=3e38), dict(cap=1e-44), dict(cap=3e38), dict(scale=1e-30, cap=1e20),
+    dict(cap=-1.0), dict(cap=float("nan")), dict(causal=2), dict(prefix=64),
     dict(o=4096), dict(o=8192), dict(q=4104), dict(o=16386), dict(q_stride=(1024, 516, 64)),
     dict(q_stride=(1024, 0, 64)), dict(k_stride=(1024, 128, 0)), dict(k_stride=(1024, -128, 64)),
     dict(o_stride=(0, 512, 64)), dict(v_stride=(1028, 128, 64)), dict(key_range=4100), dict(Sk=(1 << 30) + 1),

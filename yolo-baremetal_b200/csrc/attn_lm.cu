@@ -1114,9 +1114,9 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the pieces of a tile that was cut between CTAs of the split mode.
 // Block c finds the tile, if any, whose last piece is CTA c's first and which
 // began before; its pieces lie in CTAs c0 .. c (a CTA's piece that begins the
-// tile in slot 1, later ones in slot 0).  One warp per row, pieces in order.
+// tile in slot 1, later ones in slot 0).  One warp per row.
 template <typename T>
-__global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ AttnPlan p) {
+__global__ void __launch_bounds__(1024) attn_join_kernel(const __grid_constant__ AttnPlan p) {
   const yb_attn_args& a = p.a;
   const int c = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Walk w;
@@ -1130,31 +1130,44 @@ __global__ void __launch_bounds__(256) attn_join_kernel(const __grid_constant__ 
   while (c0 > 0 && w.total * c0 / w.ctas > u0) --c0;
   const int q_len = clamp_len(a.q_len, s.b, a.Sq);
   const size_t slot_size = static_cast<size_t>(p.rows) * (a.D + 4);
-  for (int row = warp; row < p.rows; row += 8) {
+  const int pieces = c - c0 + 1;
+  for (int row = warp; row < p.rows; row += blockDim.x >> 5) {
     const int x = static_cast<int>(p.fd_gp.div(row)), i = s.qt * p.np + x, h = s.hg * p.gp + row - x * p.gp;
     if (i >= q_len) break;
+    // A lane per piece for maxima and sums, then all lanes on each piece's row.
+    auto piece_ml = [&](int k) {
+      const float* sl = p.ws + (2 * static_cast<size_t>(c0 + k) + (k == 0)) * slot_size;
+      return *reinterpret_cast<const float2*>(sl + static_cast<size_t>(p.rows) * a.D + 2 * row);
+    };
     float m = -INFINITY;
-    for (int k = c0; k <= c; ++k) {
-      const float* ml = p.ws + (2 * static_cast<size_t>(k) + (k == c0)) * slot_size + static_cast<size_t>(p.rows) * a.D;
-      m = fmaxf(m, ml[2 * row]);
-    }
+    for (int k = lane; k < pieces; k += 32) m = fmaxf(m, piece_ml(k).x);
+    for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
     const float mb = m == -INFINITY ? 0.f : m;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const int d = 4 * lane;
-    for (int k = c0; k <= c; ++k) {
-      const float* sl = p.ws + (2 * static_cast<size_t>(k) + (k == c0)) * slot_size;
-      const float2 ml = *reinterpret_cast<const float2*>(sl + static_cast<size_t>(p.rows) * a.D + 2 * row);
-      const float f = ex2_ftz(ml.x - mb);
-      l = fmaf(ml.y, f, l);
-      if (d < a.D) {
-        const float4 v = *reinterpret_cast<const float4*>(sl + static_cast<size_t>(row) * a.D + d);
-        o.x = fmaf(v.x, f, o.x);
-        o.y = fmaf(v.y, f, o.y);
-        o.z = fmaf(v.z, f, o.z);
-        o.w = fmaf(v.w, f, o.w);
+    for (int k0 = 0; k0 < pieces; k0 += 32) {
+      const int n = min(32, pieces - k0);
+      float f = 0.f;
+      if (lane < n) {
+        const float2 ml = piece_ml(k0 + lane);
+        f = ex2_ftz(ml.x - mb);
+        l = fmaf(ml.y, f, l);
+      }
+#pragma unroll 4
+      for (int k = 0; k < n; ++k) {
+        const float w = __shfl_sync(0xFFFFFFFFu, f, k);
+        if (d < a.D) {
+          const float* sl = p.ws + (2 * static_cast<size_t>(c0 + k0 + k) + (k0 + k == 0)) * slot_size;
+          const float4 v = *reinterpret_cast<const float4*>(sl + static_cast<size_t>(row) * a.D + d);
+          o.x = fmaf(v.x, w, o.x);
+          o.y = fmaf(v.y, w, o.y);
+          o.z = fmaf(v.z, w, o.z);
+          o.w = fmaf(v.w, w, o.w);
+        }
       }
     }
+    for (int x0 = 16; x0; x0 >>= 1) l += __shfl_xor_sync(0xFFFFFFFFu, l, x0);
     const float inv = l == 0.f ? 0.f : 1.0f / l;
     if (d < a.D)
       *reinterpret_cast<uint2*>(static_cast<T*>(a.o) + s.b * a.o_stride[0] + static_cast<long long>(i) * a.o_stride[1] +
@@ -1235,9 +1248,19 @@ AttnPlan plan_attn(const yb_attn_args& a, int num_sms) {
   p.fd_gp = FastDiv(static_cast<uint32_t>(p.gp));
   const long long segs = static_cast<long long>(a.B) * p.tiles * p.groups;
   const int blocks = (a.Sk + kB - 1) / kB;
+  // Keys are cut where tiles do not fill the SMs (16 heads on 4, D 128, us cut /
+  // in row mode: 960 rows over 8,000 keys 107 / 122, 384 over 8,000 66 / 121,
+  // 64 rows of 8 heads on one over 30,000 85 / 416).
   p.split = p.tiles == 1 || segs <= num_sms;
   if (p.split) {
-    p.whole = blocks <= 4;
+    // Short tiles stay whole and need no join: up to 4 blocks (one token over
+    // 500 keys, 16 sequences: 16.6 against 20.8 with cuts), up to 8 once there
+    // are tiles for a good part of the SMs (64 sequences of 900 keys 45 against
+    // 62, 800 rows of a prompt 23 against 47; but one sequence of 1,000 keys 22
+    // against 19).
+    p.whole = blocks <= 4 || (blocks <= 8 && segs >= 32);
+    // A CTA's least share: with 8 blocks instead of 4 one sequence of 2,000 keys
+    // takes 26 us instead of 21, with 2 as long.
     p.unit_min = 4;
     const long long most = p.whole ? segs : segs * blocks;
     p.grid = static_cast<int>(most < num_sms ? most : num_sms);
@@ -1282,9 +1305,9 @@ cudaError_t launch_attn(const AttnPlan& p, cudaStream_t s) {
                          return cudaGetLastError();
                        });
   if (e != cudaSuccess || !p.split || p.whole) return e;
-  const dim3 grid(static_cast<unsigned>(p.grid));
-  if (a.dtype == YB_F16) return launch_pdl(attn_join_kernel<__half>, grid, dim3(256), 0, s, p);
-  return launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, p);
+  const dim3 grid(static_cast<unsigned>(p.grid)), block(static_cast<unsigned>(32 * (p.rows < 32 ? p.rows : 32)));
+  if (a.dtype == YB_F16) return launch_pdl(attn_join_kernel<__half>, grid, block, 0, s, p);
+  return launch_pdl(attn_join_kernel<__nv_bfloat16>, grid, block, 0, s, p);
 }
 
 }  // namespace yb

@@ -42,6 +42,9 @@ status_t check_sizes(const yb_attn_args& a) {
     return bad("at most 2^30 keys and 2^31 - 1 rows times heads");
   if (!std::isfinite(a.scale) || !(a.scale > 0.f)) return bad("scale must be finite and > 0");
   if (!std::isfinite(a.cap) || a.cap < 0.f) return bad("cap must be finite and >= 0");
+  if (!std::isfinite(a.scale * 1.5f) || !std::isfinite(a.cap * 1.5f) ||
+      (a.cap > 0.f && (!std::isfinite(a.scale / a.cap) || a.scale / a.cap == 0.f)))
+    return bad("scale, cap or scale / cap leaves the range of fp32");
   if (a.causal != 0 && a.causal != 1) return bad("causal must be 0 or 1");
   if (a.prefix && !a.causal) return bad("prefix needs causal");
   return SUCCESS;
