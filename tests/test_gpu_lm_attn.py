@@ -96,6 +96,32 @@ def test_tiles_without_keys_between_others():
         run_case(60, 3, 3000, 8, 4, 64, causal=causal, k_len=i32([6 * k for k in kl[:60]]))
 
 
+@pytest.mark.parametrize("Sk", [500, 3000])
+def test_runs_of_tiles_without_keys(Sk):
+    """Runs of sequences without a key, of every length, between ones that have some: the roles of a CTA pass the empty
+    ones at their own pace and must still meet at the others (att.check reports a wait that ran out)."""
+    import yb_ops
+
+    B = 600
+    kl = [0] * B
+    at = 0
+    for run in range(1, 30):
+        at += run % 7 + 1
+        if at < B:
+            kl[at] = (run * 911) % Sk + 1
+    for at in range(200, B, 3):
+        kl[at] = (at * 37) % Sk + 1
+    q, k, v, out = tensors(B, 1, Sk, 16, 8, 64, "bf16")
+    att = yb_ops.Attention(16, 8, 64, torch.bfloat16, causal=True)
+    want = None
+    for _ in range(30):
+        got = att(q, k, v, k_len=i32(kl))
+        want = got if want is None else want
+        assert torch.equal(got, want)
+    att.check()
+    run_case(B, 1, Sk, 4, 2, 64, causal=True, k_len=i32(kl))
+
+
 def test_prefix():
     for Sq, Sk in [(300, 300), (100, 700), (1, 400)]:
         run_case(4, Sq, Sk, 4, 2, 64, causal=True, prefix=i32([0, 1, 200, 10 ** 6]))

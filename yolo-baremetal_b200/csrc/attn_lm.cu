@@ -78,11 +78,18 @@ constexpr int kSoftmaxRegs = 200, kOtherRegs = 104;
 constexpr uint32_t kChunkBytes = kB * 128;  // 128 rows x 64 elements, 128-byte swizzle
 constexpr uint32_t kTmemCols = 512;
 constexpr float kLog2e = 1.44269504f;
-constexpr float kRaise = 8.0f;  // log2 growth of the maximum that O is rescaled for
-// Sum of a block up to which the maximum at hand serves it: fp16 weights end at
-// 65504, bf16 ones and fp32 sums near 2^127, which leaves 2^31 for keys and values.
+// A row's weights are 2^(s - m), m its reference: its maximum when that was set,
+// for fp16 less 8, so that the largest weights are 2^8 and what falls below the
+// type's normal numbers is 2^-22 of them instead of 2^-14.
 template <typename T>
-constexpr float kFits = std::is_same<T, __half>::value ? 4096.0f : 7.9228163e28f;
+constexpr float kHead = std::is_same<T, __half>::value ? 8.0f : 0.0f;
+// log2 of a weight up to which a searched maximum leaves the reference alone.
+constexpr float kRaise = 15.0f;
+// Sum of a half block up to which the reference at hand serves it: fp16 weights
+// end at 65504, bf16 ones and fp32 sums near 2^127, which leaves 2^31 for keys
+// and values.
+template <typename T>
+constexpr float kFits = std::is_same<T, __half>::value ? 32768.0f : 7.9228163e28f;
 constexpr int kSmemMax = 232448;
 constexpr int kCtlBytes = 3072;  // control block, after up to 1 KB of alignment
 
@@ -425,7 +432,7 @@ struct Ring {
 
 // ------------------------------------------------------------------ softmax
 struct RowState {
-  float m = -INFINITY, l = 0.f;
+  float m = -INFINITY, l = 0.f;  // reference of the weights (log2 units) and their sum
   int lo = 0, hi = 0, pos = 0;
   float slope = 0.f;
   bool valid = false;
@@ -467,7 +474,7 @@ struct Mask {
 };
 
 // One half block of one row: raw scores in s; the weights go to tensor memory at
-// `tp` as packed pairs, the row's maximum (log2 units) and sum are brought up
+// `tp` as packed pairs, the row's reference (its maximum, log2 units) and sum are brought up
 // to date.  Returns the factor that O has to be scaled by (1: none).
 //
 // The maximum in use only has to keep weights in range, so a half block that every
@@ -583,8 +590,9 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   }
   float factor = 1.0f;
   if (first) {
-    r.m = m;
-  } else if (m > r.m + (fits ? kRaise : 0.f)) {
+    r.m = m - kHead<T>;
+  } else if (m > r.m + (fits ? kRaise : kHead<T>)) {
+    m -= kHead<T>;
     factor = ex2_ftz(r.m - m);
     r.l *= factor;
     r.m = m;
@@ -740,6 +748,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------------------------------------- UMMAs
     Ring rg;
     uint32_t p_phase[2] = {0, 0}, q_phase = 0;  // of a pipeline, both halves
+    // Pieces with keys.  The others move no barrier, in any role: a role that
+    // passed through them alone would get two phases ahead of another's wait.
     int piece = 0;
     bool ok = true, q_open = false;
     const uint32_t id_s = idesc_f32<T>(kH, false), id_o = idesc_f32<T>(16 * ksteps, true);
@@ -873,13 +883,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (n + 1 < steps) drop(n + 1, ks);
           }
         }
-      } else if (SPLIT && piece > 0) {
-        // Once a piece also where there is nothing to do: a wait two phases
-        // behind would pass on the parity of an earlier one.
-        wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty);
+        ++piece;
       }
       if (!ok) break;
-      ++piece;
       if constexpr (SPLIT)
         more = walk.next(p, &pc);
       else
@@ -997,19 +1003,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       float w[2] = {1.f, 0.f}, m = st.m, l = st.l;
       bool have[2] = {done > 0, false};
+      const bool work = r.j1[0] > r.j0[0];  // split mode: the piece has keys
       if constexpr (SPLIT) {
         if (t == 1) {
-          if (piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
-          C.ml[row] = make_float2(st.m, st.l);
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&C.ml_full);
-          ++piece;
+          if (work) {
+            if (piece > 0 && !wait(&C.o_empty, (piece - 1) & 1, kErrWaitAccEmpty)) break;
+            C.ml[row] = make_float2(st.m, st.l);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&C.ml_full);
+            ++piece;
+          }
           more = walk.next(p, &pc);
           continue;
         }
-        if (!wait(&C.ml_full, piece & 1, kErrWaitAccFull)) break;
-        const float2 o = C.ml[row];
+        float2 o = make_float2(-INFINITY, 0.f);
+        if (work) {
+          if (!wait(&C.ml_full, piece & 1, kErrWaitAccFull)) break;
+          o = C.ml[row];
+        }
         have[1] = r.j1[0] - r.j0[0] > 1;
         m = fmaxf(st.m, o.x);
         const float mb = m == -INFINITY ? 0.f : m;
@@ -1092,11 +1104,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
       }
-      ++piece;
       if constexpr (SPLIT) {
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(&C.o_empty);
+        if (work) {
+          if (lane == 0) mbar_arrive(&C.o_empty);
+          ++piece;
+        }
         more = walk.next(p, &pc);
       } else {
         more = false;
