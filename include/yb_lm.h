@@ -39,7 +39,8 @@ typedef enum { YB_F32 = 0, YB_F16 = 1, YB_BF16 = 2 } yb_dtype;
  * Key head h / (Hq / Hkv).  A row that sees no key gives zeros.  Rows i >=
  * q_len[b] of o keep their contents.  Keys that a row does not see do not
  * touch it, whatever they hold (infinities and NaN included).  A visible NaN
- * score, or one of +infinity, makes the row NaN. */
+ * score, or one of +infinity, makes the row NaN.  Scores, sums and o are formed
+ * in fp32; the weights enter the second product rounded to dtype. */
 typedef struct {
     const void* q; /* [B, Sq, Hq, D]  */
     const void* k; /* [B, Sk, Hkv, D] */
@@ -87,7 +88,8 @@ status_t yb_attn_debug_withhold(void* attn);
  *   y_d = x_d / sqrt(mean(x^2) + eps) * (weight_d + weight_add)
  * then pair i of the first R dimensions is rotated by the angle
  * positions[b][t] * inv_freq[i] (radians; formed and reduced to one turn in 64
- * bits): pairs (i, i + R/2), or (2i, 2i + 1) when interleaved.
+ * bits): pairs (i, i + R/2), or (2i, 2i + 1) when interleaved.  fp32 between
+ * the load and the store (a sum of squares past its range gives zeros).
  * q -> q_out[b][t]; k -> k_out[b][start[b] + t], and v, unchanged, to the same
  * row of v_out: rows of a cache.  Rows outside [0, cache_rows) are not
  * written; nothing else of the outputs is touched.  q_out may be q, and, when

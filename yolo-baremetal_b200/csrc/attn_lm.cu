@@ -91,7 +91,7 @@ constexpr float kRaise = 15.0f;
 template <typename T>
 constexpr float kFits = std::is_same<T, __half>::value ? 32768.0f : 7.9228163e28f;
 constexpr int kSmemMax = 232448;
-constexpr int kCtlBytes = 3072;  // control block, after up to 1 KB of alignment
+constexpr int kCtlBytes = 3 * 1024;  // control block, after up to 1 KB of alignment
 
 template <int HDP>
 __host__ __device__ constexpr int chunks() { return HDP / 64; }
