@@ -19,20 +19,13 @@ SIZE = {"f32": 4, "f16": 2, "bf16": 2}
 GOLDEN = 0.6180339887498949
 
 
-_module = None
-
-
 def _ops():
-    global _module
-    if _module is not None:
-        return _module
     path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "yolo-baremetal_b200")
     if path not in sys.path:
         sys.path.insert(0, path)
     import yb_ops
 
-    _module = yb_ops
-    return _module
+    return yb_ops
 
 
 # ------------------------------------------------------------------ the cases
