@@ -96,11 +96,12 @@ __device__ __forceinline__ float value_of(u64 c) {
 struct Row {
   double best = 0, c = 0;  // largest logit, log2(e) / T
   float bestf = 0, cf = 0;
-  float floor = 0;  // tokens below weigh less than half a unit
+  float floor = 0;  // tokens below weigh less than half a unit, none above it is 46 octaves down
 };
 
 // rint(2^44 2^y), y = (x - best) log2(e) / T <= 0, as a whole fp64 number; only
-// for x >= floor.
+// for x >= floor (below, the exponent may wrap: the result is then any number
+// and is not used).
 // 2^y = 2^n 2^(j/64) 2^r with |r| <= 1/128 (table-driven, after Tang 1989): the
 // Taylor polynomial of degree 4 leaves (r ln 2)^5 / 120 < 2^-44.  Rounding to
 // whole numbers is done by adding 1.5 2^52 and 2^52: twelve fp64 operations and
@@ -565,8 +566,10 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
   row.best = bestf;
   row.c = 1.4426950408889634074 / static_cast<double>(temp);
   row.cf = static_cast<float>(fmin(16.0 * row.c, 1e30));
-  // 2^44 2^-45.5 < 1/2 after the rounding to fp32 too (toward -infinity).
-  row.floor = __double2float_rd(fmax(row.best - 45.5 / row.c, -static_cast<double>(FLT_MAX)));
+  // 2^44 2^-45.5 < 1/2.  Rounded up to fp32, so that the comparison with an
+  // fp32 logit is the exact one, also where one step of fp32 below the maximum
+  // is many octaves: weight_d's exponent has room for 1,000.
+  row.floor = __double2float_ru(fmax(row.best - 45.5 / row.c, -static_cast<double>(FLT_MAX)));
 
   Settings s;
   s.u = a.u[b] > 0.0f ? a.u[b] : 0.0f;
