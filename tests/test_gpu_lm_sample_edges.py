@@ -1,5 +1,7 @@
 """yb_sample where its fixed-point weights could go wrong: neighbours of the
-largest logit at small temperatures."""
+largest logit at small temperatures, and tokens of very small weight."""
+import math
+
 import numpy as np
 import pytest
 import torch
@@ -63,3 +65,22 @@ def test_every_row_gets_a_token():
         x[0, 0] = x[1, 4500] = x[2, V - 1] = np.float32(12.3)
         token, lp = run(torch.from_numpy(x).cuda(), [0.0, 0.5, 0.9999], temperature=[t] * 3)
         assert token.tolist() == [0, 4500, V - 1] and lp.tolist() == [0.0, 0.0, 0.0], t
+
+
+@pytest.mark.parametrize("octaves", [20, 30, 36, 42, 44])
+@pytest.mark.parametrize("V", [300, 3000, 50001])
+def test_log_probability_of_light_tokens(V, octaves):
+    """A peak at the last index and tokens of weight 2^-octaves before it: u = 0 takes the first of those.  Its
+    log-probability is that of its logit, not of its weight in whole units of 2^-44.
+
+    Bound: the result's rounding, half a step of 2^-24 |lp|; the whole weight, summed in units of 2^-44, is off by at
+    most V 2^-45 < 2^-27 of the peak's; 2^-22 max(1, |lp|) covers both."""
+    x = np.full((6, V), -(octaves + 0.37) * math.log(2.0), np.float32)  # no whole number of 2^-44
+    x -= np.linspace(0.0, 0.2, V, dtype=np.float32)
+    x[:, -1] = 0.0
+    for kw in ({}, dict(top_k=[V - 1, 2, 7, 40, 250, 290]), dict(min_p=[2.0 ** -46] * 6)):
+        token, lp = run(torch.from_numpy(x).cuda(), [0.0] * 6, **kw)
+        for b in range(6):
+            want, wlp = sample_ref(x[b], 0.0, **{k: v[b] for k, v in kw.items()})
+            assert want == 0 and token[b] == 0
+            assert abs(lp[b] - wlp) <= 2.0 ** -22 * max(1.0, abs(wlp)), (lp[b], wlp)

@@ -179,9 +179,13 @@ __device__ __forceinline__ u64 goal_of(float u, u64 all) {
   const u64 g = static_cast<u64>(fmin(static_cast<double>(u), 1.0) * static_cast<double>(all));
   return g < all ? g : all - 1;
 }
-__device__ __forceinline__ void answer(const yb_sample_args& a, int b, uint32_t token, u64 w, u64 all) {
+// Token of logit x.  Its log-probability comes from the logit: a weight of few
+// units of 2^-44 knows it to a few bits only.
+__device__ __forceinline__ void answer(const yb_sample_args& a, int b, uint32_t token, float x, const Row& r, u64 all) {
   a.token[b] = static_cast<int>(token);
-  if (a.logprob) a.logprob[b] = static_cast<float>(log(static_cast<double>(w) / static_cast<double>(all)));
+  if (a.logprob)
+    a.logprob[b] = static_cast<float>((static_cast<double>(x) - r.best) * r.c * 0.69314718055994530942 -
+                                      log(static_cast<double>(all) / kOne));
 }
 
 // Bins 2 t and 2 t + 1 of thread t: what lies before each, and the sums of all.
@@ -462,13 +466,16 @@ struct Picker {
     if (t == kept - 1) F.rank_sum[1] = sum;
     // By rising index: the composite's low half is ~index.
     F.l.list[t] = w;
+    F.cnt[t] = __float_as_uint(value_of(c));
     const u64 by_index = sort(t < kept ? (c << 32) | static_cast<uint32_t>(t) : 0ull, kept);
     __syncthreads();
     const u64 all = F.rank_sum[1];
     const u64 wi = t < kept ? F.l.list[static_cast<uint32_t>(by_index)] : 0ull;
     const u64 upto = scan(wi);
     const u64 goal = goal_of(s.u, all);
-    if (t < kept && upto > goal && upto - wi <= goal) answer(a, b, 0xFFFFFFFFu - static_cast<uint32_t>(by_index >> 32), wi, all);
+    if (t < kept && upto > goal && upto - wi <= goal)
+      answer(a, b, 0xFFFFFFFFu - static_cast<uint32_t>(by_index >> 32),
+             __uint_as_float(F.cnt[static_cast<uint32_t>(by_index)]), row, all);
   }
 };
 
@@ -672,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
     const u64 w = static_cast<u64>(kept(j));
     run_sum += w;
     if (run_sum > goal) {
-      answer(a, b, first + j - pad, w, all);
+      answer(a, b, first + j - pad, raw[j], row, all);
       return;
     }
   }
