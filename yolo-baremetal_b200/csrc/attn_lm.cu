@@ -439,23 +439,34 @@ struct RowState {
 };
 
 struct ScoreConst {
-  float sc2;         // scale * log2(e); with a cap: scale / cap
-  float cap2;        // cap * log2(e)
-  float c0, c1, c2;  // cap2 tanh(sc2 s) = s (c0 + c1 s^2 + c2 s^4) for |s| <= near
+  float sc2;             // scale * log2(e); with a cap: scale / cap
+  float cap2;            // cap * log2(e)
+  float c0, c1, c2, c3;  // cap2 tanh(sc2 s) = s (c0 + c1 s^2 + c2 s^4 + c3 s^6) for |s| <= near
   float near, near2;
   bool forward;  // causal without prefix: no visible key lies behind its row
 };
 
 __device__ __forceinline__ float2 both(float x) { return make_float2(x, x); }
 
-// cap2 tanh(sc2 s) for any s: 1 - 2 / (1 + e^(2u)).
-__device__ __forceinline__ float cap_any(float s, const ScoreConst& c) {
-  return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(s * (c.sc2 * (2.0f * kLog2e)))), 1.0f);
-}
-// c0 + c1 z + c2 z^2 with z = s^2, for a pair.
+// tanh(u) / u = 1 + k1 u^2 + k2 u^4 + k3 u^6 on |u| <= kNear, relative error
+// 7.0e-8 (1.2 units of 2^-24): least maximum relative error with the first
+// coefficient held at 1 (Remez exchange).
+constexpr float kNear = 0.375f;
+constexpr float kTanh1 = -0.333323335f, kTanh2 = 0.132897262f, kTanh3 = -0.0484872926f;
+
+// c0 + c1 z + c2 z^2 + c3 z^3 with z = s^2, for a pair.
 __device__ __forceinline__ float2 cap_poly(float2 z, const ScoreConst& c) {
-  const float2 q = __ffma2_rn(both(c.c2), z, both(c.c1));
+  const float2 q = __ffma2_rn(__ffma2_rn(both(c.c3), z, both(c.c2)), z, both(c.c1));
   return __ffma2_rn(q, z, both(c.c0));
+}
+// cap2 tanh(sc2 s) for any s: the polynomial where it holds (the other form
+// loses there what the subtraction cancels: its error is one of the cap, not of
+// the score), else 1 - 2 / (1 + e^(2u)).
+__device__ __forceinline__ float2 cap_any(float2 s, const ScoreConst& c) {
+  const float k = fminf(c.sc2 * (2.0f * kLog2e), 3.4028234e38f);  // finite: 0 times it is 0
+  auto large = [&](float x) { return c.cap2 * fmaf(-2.0f, rcp_ftz(1.0f + ex2_ftz(x * k)), 1.0f); };
+  const float2 small = __fmul2_rn(cap_poly(__fmul2_rn(s, s), c), s);
+  return make_float2(fabsf(s.x) <= c.near ? small.x : large(s.x), fabsf(s.y) <= c.near ? small.y : large(s.y));
 }
 
 // Column e of a half block that begins at key0 is visible.
@@ -484,9 +495,14 @@ struct Mask {
 // left the range.  Only then and in a row's first half block is the maximum
 // searched.
 //
-// cap tanh(s / cap) is a polynomial on the FMA pipe while all scores lie within
-// 3/8 of the cap (error 8e-7 of the cap), else 1 - 2 / (1 + e^2u), with two
-// more steps of the exponential pipe that bounds the sweep.
+// cap tanh(s / cap) is a polynomial on the FMA pipe while all scores of the
+// warp's rows lie within 3/8 of the cap, else cap_any, with two more steps of
+// the exponential pipe that bounds the sweep.  Either is within 16 2^-24 of the
+// capped score, less than the 32-bit dot product before it (a polynomial two
+// coefficients shorter was off by 8e-7 of the cap: 2 x 4,096 capped rows 154 us
+// instead of 158).  Where scores are capped outside the first try they are so
+// in place, ahead of the sweep: inside it, 24 sequences of up to 16,384 keys
+// took 221 us instead of 205.
 template <typename T, bool CAP, bool BIAS>
 __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& r, const ScoreConst& c, int key0,
                                                bool masked, bool first) {
@@ -544,7 +560,7 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   }
 
   const Mask vis(key0, r.lo, r.hi);
-  bool near = true;  // every visible score of the warp's rows within half the cap
+  bool near = true;  // every visible score of the warp's rows within 3/8 of the cap
   if constexpr (CAP) {
     if (masked) {  // NaN takes no part in minima and maxima
 #pragma unroll
@@ -564,7 +580,11 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
         }
       } else {
 #pragma unroll
-        for (int e = 0; e < kH; ++e) s[e] = cap_any(s[e], c);
+        for (int e = 0; e < kH; e += 2) {
+          const float2 y = cap_any(make_float2(s[e], s[e + 1]), c);
+          s[e] = y.x;
+          s[e + 1] = y.y;
+        }
       }
     }
     const float mul = CAP ? 1.0f : c.sc2;
@@ -583,7 +603,7 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   float m = fmaxf(max_of(s), -INFINITY);
   if constexpr (!BIAS) {
     if constexpr (CAP) {
-      if (m > -INFINITY) m = cap_any(m, c);
+      if (m > -INFINITY) m = cap_any(make_float2(m, m), c).x;
     } else {
       m *= c.sc2;
     }
@@ -601,11 +621,26 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   if constexpr (BIAS) {
     r.l += sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
   } else if constexpr (CAP) {
-    r.l += sweep([&](float2 x, int e) {
-      const float2 y = near ? __ffma2_rn(cap_poly(__fmul2_rn(x, x), c), x, base)
-                            : make_float2(cap_any(x.x, c) + base.x, cap_any(x.y, c) + base.y);
-      return masked ? make_float2(vis[e] ? y.x : -INFINITY, vis[e + 1] ? y.y : -INFINITY) : y;
-    });
+    if (near) {
+#pragma unroll
+      for (int e = 0; e < kH; e += 2) {
+        const float2 x = make_float2(s[e], s[e + 1]), y = __fmul2_rn(cap_poly(__fmul2_rn(x, x), c), x);
+        s[e] = y.x;
+        s[e + 1] = y.y;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < kH; e += 2) {
+        const float2 y = cap_any(make_float2(s[e], s[e + 1]), c);
+        s[e] = y.x;
+        s[e + 1] = y.y;
+      }
+    }
+    if (masked) {
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
+    }
+    r.l += sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
   } else {
     r.l += sweep([&](float2 x, int) { return __ffma2_rn(x, both(c.sc2), base); });
   }
@@ -911,17 +946,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     if constexpr (CAP) {
       c.sc2 = a.scale / a.cap;
       c.cap2 = a.cap * kLog2e;
-      // Least maximum absolute error fit of tanh(u) / u in u^2 on |u| <= 3/8,
-      // for s = u / sc2; no polynomial where its coefficients could leave fp32.
+      // The polynomial in s = u / sc2.  For caps of some 2^20 times the scale
+      // and more its last coefficients leave the normal numbers: it ends where
+      // the next one would count (u^2 / 3 < 2^-24 at 4e-4, and so on).
       const float k2 = c.sc2 * c.sc2;
-      c.c0 = c.cap2 * c.sc2 * 0.9999854f;
-      c.c1 = c.cap2 * c.sc2 * k2 * -0.33248851f;
-      c.c2 = c.cap2 * c.sc2 * k2 * k2 * 0.12098849f;
-      c.near = c.sc2 >= 1.0f / 4096.0f && c.sc2 <= 4096.0f ? 0.375f / c.sc2 : -1.0f;
-      c.near2 = c.near > 0.f ? c.near * c.near : -1.0f;
+      c.c0 = a.scale * kLog2e;
+      c.c1 = c.c0 * k2 * kTanh1;
+      c.c2 = c.c0 * k2 * k2 * kTanh2;
+      c.c3 = c.c0 * k2 * k2 * k2 * kTanh3;
+      const auto normal = [](float x) { return fabsf(x) >= 1.17549435e-38f; };
+      const float reach = normal(c.c3) ? kNear : normal(c.c2) ? 0.1f : normal(c.c1) ? 0.01f : 4e-4f;
+      const bool finite = fabsf(c.c1) <= 3.4028234e38f && fabsf(c.c2) <= 3.4028234e38f && fabsf(c.c3) <= 3.4028234e38f;
+      c.near = finite ? fminf(reach / c.sc2, 1.8e19f) : -1.0f;
+      c.near2 = finite ? c.near * c.near : -1.0f;
     } else {
       c.sc2 = a.scale * kLog2e;
-      c.cap2 = c.c0 = c.c1 = c.c2 = c.near = c.near2 = 0.f;
+      c.cap2 = c.c0 = c.c1 = c.c2 = c.c3 = c.near = c.near2 = 0.f;
     }
     c.forward = a.causal && !a.prefix;
     uint32_t s_phase = 0;
