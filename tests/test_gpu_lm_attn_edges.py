@@ -1,5 +1,5 @@
 """yb_attn_run where single parts of its arithmetic could go wrong: caps far from
-the scores."""
+the scores, scores of -infinity under a cap."""
 import math
 
 import pytest
@@ -94,3 +94,39 @@ def test_equal_scores_weigh_equally(scale, cap, dot, dt):
     other = cap * math.tanh(-1000.0 / cap)
     assert s - other > 30 * math.log(2.0)  # the rest weighs nothing
     assert float(out[0, 0].double().abs().max()) <= (2 * 16 * U * s + 2 * half_step(dtype)) / 2 * (1 + 2.0 ** -7)
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("slopes", [False, True])
+@pytest.mark.parametrize("Sk", [3, 64, 200, 1500])
+def test_scores_of_minus_infinity_under_a_cap(Sk, slopes, dt):
+    """tanh(-infinity) = -1: such keys weigh e^(-cap) beside a score of 0, and all alike where there are no others."""
+    import yb_ops
+
+    dtype = T[dt]
+    D, cap = 16, 2.0
+    g = torch.Generator(device="cuda").manual_seed(Sk)
+    v = torch.randn(1, Sk, 1, D, generator=g, device="cuda").to(dtype)
+    q = torch.zeros(1, 2, 1, D, device="cuda", dtype=dtype)
+    q[..., 0] = 1.0
+    sl = torch.tensor([0.01], device="cuda") if slopes else None
+    for finite in ([], [0], [Sk - 1], [Sk // 2]):
+        k = torch.zeros(1, Sk, 1, D, device="cuda", dtype=dtype)
+        k[..., 0] = -math.inf
+        for j in finite:
+            k[0, j, 0, 0] = 0.0
+        att = yb_ops.Attention(1, 1, D, dtype, cap=cap)
+        out = att(q, k, v, slopes=sl)
+        att.check()
+        s = torch.full((2, Sk), -cap, dtype=torch.float64, device="cuda")
+        for j in finite:
+            s[:, j] = 0.0
+        if slopes:
+            row = torch.arange(2, device="cuda")[:, None] + Sk - 2
+            s -= 0.01 * (row - torch.arange(Sk, device="cuda")).abs().double()
+        p = torch.softmax(s, -1)
+        want = p @ v[0, :, 0].double()
+        a = half_step(dtype)
+        e = 20 * U * (cap + 0.01 * Sk)
+        bound = (a + 4 * e + 2.0 ** -20 + 2 * Sk * U) * (p @ v[0, :, 0].double().abs()) + a * want.abs() + half_subnormal(dtype)
+        assert float(((out[0, :, 0].double() - want).abs() - bound).max()) <= 0, finite

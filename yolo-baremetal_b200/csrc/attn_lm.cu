@@ -500,9 +500,9 @@ struct Mask {
 // the exponential pipe that bounds the sweep.  Either is within 16 2^-24 of the
 // capped score, less than the 32-bit dot product before it (a polynomial two
 // coefficients shorter was off by 8e-7 of the cap: 2 x 4,096 capped rows 154 us
-// instead of 158).  Where scores are capped outside the first try they are so
+// instead of 159).  Where scores are capped outside the first try they are so
 // in place, ahead of the sweep: inside it, 24 sequences of up to 16,384 keys
-// took 221 us instead of 205.
+// took 221 us instead of 203.
 template <typename T, bool CAP, bool BIAS>
 __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& r, const ScoreConst& c, int key0,
                                                bool masked, bool first) {
@@ -560,67 +560,14 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
   }
 
   const Mask vis(key0, r.lo, r.hi);
-  bool near = true;  // every visible score of the warp's rows within 3/8 of the cap
   if constexpr (CAP) {
     if (masked) {  // NaN takes no part in minima and maxima
 #pragma unroll
       for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : __uint_as_float(0x7FC00000u);
     }
     const float far = fmaxf(fabsf(max_of(s)), fabsf(min_of(s)));
-    near = __all_sync(0xFFFFFFFFu, !(far > c.near) || !r.valid);
-  }
-  if constexpr (BIAS) {
-    if constexpr (CAP) {
-      if (near) {
-#pragma unroll
-        for (int e = 0; e < kH; e += 2) {
-          const float2 x = make_float2(s[e], s[e + 1]), y = __fmul2_rn(cap_poly(__fmul2_rn(x, x), c), x);
-          s[e] = y.x;
-          s[e + 1] = y.y;
-        }
-      } else {
-#pragma unroll
-        for (int e = 0; e < kH; e += 2) {
-          const float2 y = cap_any(make_float2(s[e], s[e + 1]), c);
-          s[e] = y.x;
-          s[e + 1] = y.y;
-        }
-      }
-    }
-    const float mul = CAP ? 1.0f : c.sc2;
-    if (linear) {
-#pragma unroll
-      for (int e = 0; e < kH; ++e) s[e] = fmaf(r.slope, d0 + static_cast<float>(e), s[e] * mul);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kH; ++e) s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), s[e] * mul);
-    }
-  }
-  if (masked && (!CAP || BIAS)) {
-#pragma unroll
-    for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
-  }
-  float m = fmaxf(max_of(s), -INFINITY);
-  if constexpr (!BIAS) {
-    if constexpr (CAP) {
-      if (m > -INFINITY) m = cap_any(make_float2(m, m), c).x;
-    } else {
-      m *= c.sc2;
-    }
-  }
-  float factor = 1.0f;
-  if (first) {
-    r.m = m - kHead<T>;
-  } else if (m > r.m + (fits ? kRaise : kHead<T>)) {
-    m -= kHead<T>;
-    factor = ex2_ftz(r.m - m);
-    r.l *= factor;
-    r.m = m;
-  }
-  const float2 base = both(r.m == -INFINITY ? 0.f : -r.m);
-  if constexpr (BIAS) {
-    r.l += sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
-  } else if constexpr (CAP) {
+    // Every visible score of the warp's rows lies within 3/8 of the cap.
+    const bool near = __all_sync(0xFFFFFFFFu, !(far > c.near) || !r.valid);
     if (near) {
 #pragma unroll
       for (int e = 0; e < kH; e += 2) {
@@ -636,10 +583,34 @@ __device__ __forceinline__ float softmax_block(float* s, uint32_t tp, RowState& 
         s[e + 1] = y.y;
       }
     }
-    if (masked) {
+  }
+  if constexpr (BIAS) {
+    const float mul = CAP ? 1.0f : c.sc2;
+    if (linear) {
 #pragma unroll
-      for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
+      for (int e = 0; e < kH; ++e) s[e] = fmaf(r.slope, d0 + static_cast<float>(e), s[e] * mul);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kH; ++e) s[e] = fmaf(-r.slope, fabsf(d0 + static_cast<float>(e)), s[e] * mul);
     }
+  }
+  if (masked) {
+#pragma unroll
+    for (int e = 0; e < kH; ++e) s[e] = vis[e] ? s[e] : -INFINITY;
+  }
+  float m = fmaxf(max_of(s), -INFINITY);
+  if constexpr (!CAP && !BIAS) m *= c.sc2;
+  float factor = 1.0f;
+  if (first) {
+    r.m = m - kHead<T>;
+  } else if (m > r.m + (fits ? kRaise : kHead<T>)) {
+    m -= kHead<T>;
+    factor = ex2_ftz(r.m - m);
+    r.l *= factor;
+    r.m = m;
+  }
+  const float2 base = both(r.m == -INFINITY ? 0.f : -r.m);
+  if constexpr (CAP || BIAS) {
     r.l += sweep([&](float2 x, int) { return __fadd2_rn(x, base); });
   } else {
     r.l += sweep([&](float2 x, int) { return __ffma2_rn(x, both(c.sc2), base); });
