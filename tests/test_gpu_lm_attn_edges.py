@@ -1,11 +1,12 @@
 """yb_attn_run where single parts of its arithmetic could go wrong: caps far from
-the scores, scores of -infinity under a cap."""
+the scores, scores of -infinity under a cap, and rows that are computed again
+because of a value that is not finite."""
 import math
 
 import pytest
 import torch
 
-from lm_util import half_step, half_subnormal
+from lm_util import attention_ref, check_attention, half_step, half_subnormal
 
 pytestmark = pytest.mark.gpu
 
@@ -130,3 +131,53 @@ def test_scores_of_minus_infinity_under_a_cap(Sk, slopes, dt):
         e = 20 * U * (cap + 0.01 * Sk)
         bound = (a + 4 * e + 2.0 ** -20 + 2 * Sk * U) * (p @ v[0, :, 0].double().abs()) + a * want.abs() + half_subnormal(dtype)
         assert float(((out[0, :, 0].double() - want).abs() - bound).max()) <= 0, finite
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("cap,slopes", [(0.0, False), (20.0, False), (0.0, True), (20.0, True)])
+def test_rows_computed_again(cap, slopes, causal, dt):
+    """A NaN in one dimension of some values: rows that see it have it there, their other dimensions as ever."""
+    import yb_ops
+
+    dtype = T[dt]
+    for n, (B, Sq, Sk, Hq, Hkv, D) in enumerate([(1, 200, 200, 4, 2, 64), (2, 3, 700, 8, 2, 128), (3, 1, 33, 2, 1, 8),
+                                                  (1, 130, 1500, 3, 1, 72), (160, 2, 300, 1, 1, 40)]):
+        g = torch.Generator(device="cuda").manual_seed(n)
+        q, k, v, out = (torch.randn(B, s, h, D, generator=g, device="cuda").to(dtype)
+                        for s, h in ((Sq, Hq), (Sk, Hkv), (Sk, Hkv), (Sq, Hq)))
+        v[:, Sk // 2, :, 5] = math.nan
+        v[:, 1, :, 0] = math.nan
+        kw = {"slopes": torch.tensor([2.0 ** -(h + 3) for h in range(Hq)], device="cuda") if slopes else None}
+        if n == 1:
+            kw["k_len"] = torch.tensor([700, 351], dtype=torch.int32, device="cuda")
+        if n == 3 and causal:
+            kw["prefix"] = torch.tensor([800], dtype=torch.int32, device="cuda")
+        before = out.clone()
+        att = yb_ops.Attention(Hq, Hkv, D, dtype, cap=cap, causal=causal)
+        att(q, k, v, out=out, **kw)
+        att.check()
+        check_attention(out, before, attention_ref(q, k, v, att.scale, cap, causal, dt=dtype, **kw))
+        assert bool(out.isnan().any())
+
+
+def test_rows_computed_again_over_many_keys():
+    """160 sequences of 300,000 keys (one tensor for all) and 128 rows, a NaN seen by every row: two tiles to a CTA, whose
+    other roles wait while the first one's rows are computed again (32 rows of a warp, once 0.23 us a key: 2.2 s, where
+    a wait gives up after 2)."""
+    import yb_ops
+
+    B, Sq, Sk, D = 160, 128, 300000, 8
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q = torch.randn(B, Sq, 1, D, generator=g, device="cuda").bfloat16()
+    k = torch.randn(1, Sk, 1, D, generator=g, device="cuda").bfloat16().expand(B, -1, -1, -1)
+    v = torch.ones(1, Sk, 1, D, device="cuda").bfloat16()
+    v[:, 0, :, 5] = math.nan
+    att = yb_ops.Attention(1, 1, D, torch.bfloat16)
+    out = att(q, k, v.expand(B, -1, -1, -1))
+    att.check()
+    nan = torch.isnan(out)
+    assert bool(nan[..., 5].all()) and int(nan.sum()) == B * Sq
+    # Values of 1 average to 1; sums of Sk positive terms in 32 bits on either side.
+    rest = torch.cat((out[..., :5], out[..., 6:]), -1).double()
+    assert float((rest - 1).abs().max()) <= 2 * Sk * U + half_step(torch.bfloat16)
