@@ -181,3 +181,49 @@ def test_rows_computed_again_over_many_keys():
     # Values of 1 average to 1; sums of Sk positive terms in 32 bits on either side.
     rest = torch.cat((out[..., :5], out[..., 6:]), -1).double()
     assert float((rest - 1).abs().max()) <= 2 * Sk * U + half_step(torch.bfloat16)
+
+
+@pytest.mark.parametrize("Sq,Sk", [(1, 2), (1, 100), (200, 300), (1, 5000), (3, 20000)])
+def test_values_near_the_end_of_the_range(Sq, Sk):
+    """Averages of bf16 values of 3e38 are such values, though their sum is past 32 bits."""
+    import yb_ops
+
+    g = torch.Generator(device="cuda").manual_seed(Sk)
+    q = torch.randn(1, Sq, 2, 64, generator=g, device="cuda").bfloat16()
+    k = torch.randn(1, Sk, 1, 64, generator=g, device="cuda").bfloat16()
+    v = torch.full((1, Sk, 1, 64), 3e38, device="cuda").bfloat16()
+    v[..., 1] *= -1
+    v[..., 2] = 1.0
+    v[..., 3] = torch.randn(1, Sk, 1, generator=g, device="cuda").bfloat16() * 1e37
+    att = yb_ops.Attention(2, 1, 64, torch.bfloat16)
+    out = torch.zeros_like(q)
+    att(q, k, v, out=out)
+    att.check()
+    check_attention(out, out, attention_ref(q, k, v, att.scale))
+
+
+@pytest.mark.parametrize("dt", ["f16", "bf16"])
+@pytest.mark.parametrize("near_end", [False, True])
+@pytest.mark.parametrize("lead", [9, 20, 33, 34, 35, 40, 50, 60, 61, 62, 66, 66.5, 67, 80])
+def test_pieces_of_very_different_references(lead, near_end, dt):
+    """Keys of score 0 but for two, a unit apart, far above and in pieces of different CTAs: either may outgrow its
+    piece's reference by any amount, or be it, and both count.  With a value near the end of the range beside them the
+    piece is computed again, from other references."""
+    import yb_ops
+
+    dtype = T[dt]
+    Sk, D = 20000, 8
+    q = torch.zeros(1, 1, 1, D, device="cuda").to(dtype)
+    q[..., 0] = 1.0
+    for a, b in ((300, 15000), (15000, 300), (19999, 70), (130, 19900), (10000, 5000), (64, 19840)):
+        k = torch.zeros(1, Sk, 1, D, device="cuda").to(dtype)
+        v = torch.zeros(1, Sk, 1, D, device="cuda").to(dtype)
+        k[0, a, 0, 0], k[0, b, 0, 0] = lead, lead + 1
+        v[0, a], v[0, b] = 1.0, -1.0
+        if near_end and dt == "bf16":
+            v[0, a, 0, 7] = v[0, (a + 1) % Sk, 0, 7] = 3e38
+        out = torch.zeros_like(q)
+        att = yb_ops.Attention(1, 1, D, dtype, scale=1.0)
+        att(q, k, v, out=out)
+        att.check()
+        check_attention(out, out, attention_ref(q, k, v, 1.0))

@@ -85,11 +85,14 @@ template <typename T>
 constexpr float kHead = std::is_same<T, __half>::value ? 8.0f : 0.0f;
 // log2 of a weight up to which a searched maximum leaves the reference alone.
 constexpr float kRaise = 15.0f;
+// Room for the sum of a tile's pieces, at most two a CTA.
+constexpr float kJoinRoom = 8.0f;
 // Sum of a half block up to which the reference at hand serves it: fp16 weights
-// end at 65504, bf16 ones and fp32 sums near 2^127, which leaves 2^31 for keys
-// and values.
+// end at 65504; bf16 ones may be 2^50 above it.  Between references 88 octaves
+// apart a join's factor falls out of fp32 (126 less kRoom and kJoinRoom), and
+// what it drops is then below 2^-38 a half block.
 template <typename T>
-constexpr float kFits = std::is_same<T, __half>::value ? 32768.0f : 7.9228163e28f;
+constexpr float kFits = std::is_same<T, __half>::value ? 32768.0f : 1.1258999e15f;
 constexpr int kSmemMax = 232448;
 constexpr int kCtlBytes = 3 * 1024;  // control block, after up to 1 KB of alignment
 
@@ -1190,7 +1193,7 @@ __global__ void __launch_bounds__(1024) attn_join_kernel(const __grid_constant__
     float m = -INFINITY;
     for (int k = lane; k < pieces; k += 32) m = fmaxf(m, piece_ml(k).x);
     for (int d = 16; d; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, d));
-    const float mb = m == -INFINITY ? 0.f : m;
+    const float mb = (m == -INFINITY ? 0.f : m) + kJoinRoom;
     float l = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
     const int d = 4 * lane;

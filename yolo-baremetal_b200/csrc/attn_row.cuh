@@ -33,8 +33,11 @@ __device__ __forceinline__ RowSpan row_span(const yb_attn_args& a, int b, int i,
   return s;
 }
 
-// Running softmax of a row: maximum (log2 units), sum, and the four dimensions
-// [4 lane, 4 lane + 4) of the weighted values.
+// Running softmax of a row: reference of the weights (log2 units), their sum, and
+// the four dimensions [4 lane, 4 lane + 4) of the weighted values.  The reference
+// is kRoom above the maximum, so that the sum over 2^30 keys of values near the
+// end of bf16 stays in fp32 (it is divided by a sum that is as much smaller).
+constexpr float kRoom = 30.0f;
 struct RowAcc {
   float m, l, o[4];
 };
@@ -92,7 +95,7 @@ __device__ RowAcc attn_row(const yb_attn_args& a, int b, int i, int h, int pos, 
     }
     float m = s;  // a NaN score is passed over here and enters the sums
     for (int x = 16; x; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xFFFFFFFFu, m, x));
-    m = fmaxf(r.m, m);
+    m = fmaxf(r.m, m + kRoom);
     const float base = m == -INFINITY ? 0.f : m;
     const float c = exp2f(r.m - base), p = lane < n ? exp2f(s - base) : 0.f;
     float sum = p;
