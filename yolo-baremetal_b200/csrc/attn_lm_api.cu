@@ -37,7 +37,9 @@ status_t check_sizes(const yb_attn_args& a) {
   if (a.Hq % a.Hkv) return bad("Hq must be a multiple of Hkv");
   if (a.D < 8 || a.D > kAttnMaxD || a.D % 8) return bad("D must be a multiple of 8 in [8, 128]");
   if (a.dtype != YB_F16 && a.dtype != YB_BF16) return bad("dtype must be YB_F16 or YB_BF16");
-  if (a.Sk > (1 << 30) || a.Sq > (1 << 30) || static_cast<long long>(a.B) * a.Sq * a.Hq > INT_MAX ||
+  // Rows first: the product of all three may pass 64 bits.
+  const long long rows = static_cast<long long>(a.B) * a.Sq;
+  if (a.Sk > (1 << 30) || a.Sq > (1 << 30) || rows > INT_MAX || rows * a.Hq > INT_MAX ||
       static_cast<long long>(a.B) * a.Hkv > (1 << 30))
     return bad("at most 2^30 keys and 2^31 - 1 rows times heads");
   if (!std::isfinite(a.scale) || !(a.scale > 0.f)) return bad("scale must be finite and > 0");
