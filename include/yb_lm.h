@@ -12,8 +12,9 @@
  * (a cudaStream_t; NULL = the default stream) and do not synchronize; they can
  * be captured into a CUDA graph once one call has run on the device before
  * (which loads the kernels).  Strides are in elements and non-negative, given
- * as [batch, row, head]; the last dimension is contiguous.  Lengths and
- * positions are read on the device, so that a captured graph follows them. */
+ * as [batch, row, head]; the last dimension is contiguous.  Pointers lie on
+ * their elements' boundaries (others are refused).  Lengths and positions are
+ * read on the device, so that a captured graph follows them. */
 
 #include <stddef.h>
 
@@ -69,7 +70,8 @@ status_t yb_attn_workspace(void* attn, const yb_attn_args* a, size_t* bytes);
 
 /* D a multiple of 8 in [8, 128]; Hq a multiple of Hkv.  q, k, v, o 16-byte
  * aligned with strides that are multiples of 8 elements; only the batch
- * strides of q, k and v may be 0 (one tensor for all sequences).  workspace:
+ * strides of q, k and v may be 0 (one tensor for all sequences).  key_range
+ * 8-byte aligned.  workspace:
  * 16-byte aligned, at least yb_attn_workspace bytes. */
 status_t yb_attn_run(void* attn, const yb_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
 

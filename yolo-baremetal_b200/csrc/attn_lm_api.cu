@@ -106,7 +106,8 @@ extern "C" status_t yb_attn_run(void* attn, const yb_attn_args* p, void* workspa
   if (!ok(a.q, a.q_stride, a.Sq, a.Hq, false) || !ok(a.o, a.o_stride, a.Sq, a.Hq, true) ||
       (a.Sk > 0 && (!ok(a.k, a.k_stride, a.Sk, a.Hkv, false) || !ok(a.v, a.v_stride, a.Sk, a.Hkv, false))))
     return bad("q, k, v, o: 16-byte aligned, strides multiples of 8 elements; only batch strides of inputs may be 0");
-  if (a.key_range && reinterpret_cast<uintptr_t>(a.key_range) % 8) return bad("key_range must be 8-byte aligned");
+  if (!on_boundary(8, a.key_range)) return bad("key_range must be 8-byte aligned");
+  if (!on_boundary(4, a.q_len, a.k_len, a.prefix, a.slopes)) return bad("lengths, prefix and slopes: 4-byte aligned");
   if (!h) return ERROR_NULL_POINTER;
   DeviceScope scope(h->device);
   if (scope.error() != cudaSuccess) return cuda_status(scope.error(), "cudaSetDevice");

@@ -6,6 +6,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <cstddef>
 #include <cstdint>
 
 #include "runtime.h"
@@ -30,6 +31,13 @@ template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// Every pointer (null ones included) lies on a boundary of `bytes`: a device
+// load off its element's boundary is a fault.
+template <typename... P>
+bool on_boundary(size_t bytes, const P*... p) {
+  return ((reinterpret_cast<uintptr_t>(p) % bytes == 0) && ...);
+}
 
 class DeviceScope {
  public:

@@ -329,6 +329,11 @@ extern "C" status_t yb_qk_norm_rope(const yb_qk_args* p, void* stream) {
   if (a.Hkv == 0) a.k = a.v = nullptr, a.k_out = a.v_out = nullptr;
   if ((a.Hq && (!a.q || !a.q_out)) || (a.Hkv && (!a.k || !a.k_out)) || (a.R && !a.inv_freq) || !a.v != !a.v_out)
     return ERROR_NULL_POINTER;
+  if (!on_boundary(a.dtype == YB_F32 ? 4 : 2, a.q, a.k, a.v, a.q_out, a.k_out, a.v_out) || !on_boundary(8, a.inv_freq) ||
+      !on_boundary(4, a.q_weight, a.k_weight, a.start, a.length, a.positions)) {
+    set_error("qk_norm_rope: a pointer is not aligned to its element");
+    return ERROR_INVALID_DIMS;
+  }
   auto same = [](const long long* x, const long long* y) { return x[0] == y[0] && x[1] == y[1] && x[2] == y[2]; };
   if ((a.Hq && a.q == a.q_out && !same(a.q_stride, a.q_out_stride)) ||
       (a.Hkv && a.k == a.k_out && (a.start || !same(a.k_stride, a.k_out_stride))) ||

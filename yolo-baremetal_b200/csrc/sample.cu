@@ -737,6 +737,11 @@ extern "C" status_t yb_sample(const yb_sample_args* a, void* stream) {
   }
   if (a->B == 0) return SUCCESS;
   if (!a->logits || !a->u || !a->token) return ERROR_NULL_POINTER;
+  if (!on_boundary(a->dtype == YB_F32 ? 4 : 2, a->logits) ||
+      !on_boundary(4, a->u, a->temperature, a->top_k, a->top_p, a->min_p, a->token, a->logprob)) {
+    set_error("sample: a pointer is not aligned to its element");
+    return ERROR_INVALID_DIMS;
+  }
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case YB_F32: return launch_sample<float>(*a, s);
