@@ -7,8 +7,9 @@
 
 Every call runs on the current torch stream of its tensors' device and does
 not synchronize; outputs that are not given are allocated.  Tensors of another
-device, type or shape than an operator takes raise ValueError, what the
-library refuses raises YBError.  The semantics stand in yb_lm.h.
+device, type or shape than an operator takes raise ValueError, as do tensors
+that require gradients outside torch.no_grad() (the operators have none); what
+the library refuses raises YBError.  The semantics stand in yb_lm.h.
 """
 from __future__ import annotations
 
@@ -55,6 +56,14 @@ def _writable(t, name: str) -> None:
     """Refuses an output whose elements share memory with one another."""
     if not t.is_contiguous() and any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
         _fail(f"{name}: an output must not be expanded")
+
+
+def _no_gradients(name: str, *tensors) -> None:
+    """Refuses tensors through which autograd would expect a gradient: the results would silently have none."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                _fail(f"{name}: no gradients; call it under torch.no_grad(), or with detached tensors")
 
 
 def _cuda(t, name: str) -> int:
@@ -129,6 +138,7 @@ class Attention:
         index, dt = self.device.index, self.dtype
         if q.dim() != 4 or k.dim() != 4:
             _fail("attention: q, k and v have four dimensions")
+        _no_gradients("attention", q, k, v, slopes, out)
         B, Sq, _, _ = q.shape
         Sk = k.shape[1]
         qs = _heads(q, "q", index, dt, (B, Sq, self.heads, self.head_dim))
@@ -174,6 +184,7 @@ def qk_norm_rope(q, k, q_weight, k_weight, inv_freq, q_out=None, k_out=None, v=N
         _fail(f"qk_norm_rope: float32, float16 or bfloat16, got {dt}")
     if q.dim() != 4 or k.dim() != 4:
         _fail("qk_norm_rope: q and k have four dimensions")
+    _no_gradients("qk_norm_rope", q, k, v, q_weight, k_weight, inv_freq, q_out, k_out, v_out)
     B, S, Hq, D = q.shape
     Hkv = k.shape[2]
     qs = _heads(q, "q", dev, dt, (B, S, Hq, D))
@@ -225,6 +236,7 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
         _fail(f"sample: float32, float16 or bfloat16, got {dt}")
     if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
         _fail("sample: logits have two dimensions, the last one contiguous")
+    _no_gradients("sample", logits, u, temperature, top_p, min_p, logprob)
     B, V = logits.shape
     i32, f32 = torch.int32, torch.float32
     if u is None:
