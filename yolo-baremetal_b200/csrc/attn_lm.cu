@@ -110,14 +110,11 @@ __host__ __device__ constexpr int smem_bytes() {
   return q_bytes<HDP, SPLIT>() + stages<HDP, SPLIT>() * chunks<HDP>() * static_cast<int>(kChunkBytes) + kCtlBytes;
 }
 
-// Control flags: a role gave up; steps of rows that are computed again.
-enum : int { kAbort = 0, kAlive = 1 };
-
 struct Ctl {
   uint64_t q_full, s_full[2][2], p_full[2][2], o_full[2][2], o_empty, ml_full, drain;
   uint64_t kv_full[8], kv_empty[8];
   uint32_t tmem;
-  int flags[2];  // kAbort, kAlive
+  int abort;
   float2 ml[kB];  // split: second pipeline's maximum and sum
 };
 static_assert(sizeof(Ctl) + 1024 <= kCtlBytes, "control block plus alignment");
@@ -421,29 +418,9 @@ __device__ __forceinline__ Blocks block_range(const AttnPlan& p, const Piece& s)
   return r;
 }
 
-__device__ __forceinline__ void raise_error(int* err, volatile int* flags, int code) {
-  flags[kAbort] = 1;
+__device__ __forceinline__ void raise_error(int* err, volatile int* abort_flag, int code) {
+  *abort_flag = 1;
   atomicCAS(err, 0, code);
-}
-
-// mbar_wait whose bound begins anew while rows are computed again, which the
-// other roles wait for and which takes as long as they have keys.  (A warp's 32
-// rows over 170,000 keys each took longer than the bound; now 32 keys at a time.)
-__device__ __forceinline__ bool bar_wait(uint64_t* bar, uint32_t parity, volatile int* flags, uint64_t limit_ns) {
-  if (mbar_try_wait(bar, parity)) return true;
-  uint64_t t0 = globaltimer_ns();
-  int alive = 0;
-  const uint32_t hint = limit_ns < 1000000u ? static_cast<uint32_t>(limit_ns) : 1000000u;
-  while (true) {
-    if (mbar_try_wait_sleep(bar, parity, hint)) return true;
-    if (flags[kAbort]) return false;
-    if (globaltimer_ns() - t0 > limit_ns) {
-      const int now = flags[kAlive];
-      if (now == alive) return false;
-      alive = now;
-      t0 = globaltimer_ns();
-    }
-  }
 }
 
 // Position in the ring of key and value blocks.
@@ -657,7 +634,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* ring = base + q_bytes<HDP, SPLIT>();
   Ctl& C = *reinterpret_cast<Ctl*>(ring + NST * kBlockBytes);
   const int warp = uni(threadIdx.x >> 5), lane = threadIdx.x & 31;
-  volatile int* flags = C.flags;
+  volatile int* abort_flag = &C.abort;
   const yb_attn_args& a = p.a;
 
   Piece pc;
@@ -696,7 +673,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&C.kv_full[i], 1);
       mbar_init(&C.kv_empty[i], 1);
     }
-    C.flags[kAbort] = C.flags[kAlive] = 0;
+    C.abort = 0;
     mbar_fence_init();
     prefetch_tmap(&tmq);
     prefetch_tmap(&tmk);
@@ -737,8 +714,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       if (lane == 0) {
         auto load = [&](const CUtensorMap* m, int bmul, int j) {
-          if (!bar_wait(&C.kv_empty[rg.slot], rg.phase ^ 1u, flags, p.wait_ns)) {
-            if (!flags[kAbort]) raise_error(p.err, flags, kErrWaitEmpty);
+          if (!mbar_wait(&C.kv_empty[rg.slot], rg.phase ^ 1u, abort_flag, p.wait_ns)) {
+            if (!*abort_flag) raise_error(p.err, abort_flag, kErrWaitEmpty);
             ok = false;
             return;
           }
@@ -766,7 +743,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         more = false;
     }
     // After an abort, copies may still be landing in shared memory.
-    if (lane == 0 && flags[kAbort]) {
+    if (lane == 0 && *abort_flag) {
       int dummy = 0;
       const int open = loads < NST ? loads : NST;
       for (int i = 0; i < open; ++i) {
@@ -788,8 +765,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t q_tx = static_cast<uint32_t>(NCH * 128 * fill);
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       // The lanes agree, so that none is left behind at a warp barrier.
-      if (ok && !__all_sync(0xFFFFFFFFu, bar_wait(bar, phase, flags, p.wait_ns))) {
-        if (lane == 0 && !flags[kAbort]) raise_error(p.err, flags, code);
+      if (ok && !__all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, p.wait_ns))) {
+        if (lane == 0 && !*abort_flag) raise_error(p.err, abort_flag, code);
         ok = false;
       }
       return ok;
@@ -928,7 +905,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int dummy = 0;
       if (q_open) mbar_wait(&C.q_full, q_phase, &dummy, p.wait_ns);
       tc_commit(&C.drain);
-      if (!mbar_wait(&C.drain, 0, &dummy, p.wait_ns)) raise_error(p.err, flags, kErrDrain);
+      if (!mbar_wait(&C.drain, 0, &dummy, p.wait_ns)) raise_error(p.err, abort_flag, kErrDrain);
     }
     __syncwarp();
   }
@@ -966,8 +943,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     auto wait = [&](uint64_t* bar, uint32_t phase, int code) {
       // The lanes agree, so that none is left behind at a warp barrier.
-      if (ok && !__all_sync(0xFFFFFFFFu, bar_wait(bar, phase, flags, p.wait_ns))) {
-        if (lane == 0 && !flags[kAbort]) raise_error(p.err, flags, code);
+      if (ok && !__all_sync(0xFFFFFFFFu, mbar_wait(bar, phase, abort_flag, p.wait_ns))) {
+        if (lane == 0 && !*abort_flag) raise_error(p.err, abort_flag, code);
         ok = false;
       }
       return ok;
@@ -1125,7 +1102,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             lo = max(lo, r.j0[0] * kB);
             hi = min(hi, r.j1[0] * kB);
           }
-          const RowAcc x = attn_row<T>(a, pc.b, wi, wh, pos, lo, hi, &C.flags[kAlive]);
+          const RowAcc x = attn_row<T>(a, pc.b, wi, wh, pos, lo, hi);
           const int d = 4 * lane, wrow = __shfl_sync(0xFFFFFFFFu, row, who);
           if (d < a.D) {
             if (part) {
