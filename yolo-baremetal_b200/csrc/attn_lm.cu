@@ -1276,17 +1276,23 @@ AttnPlan plan_attn(const yb_attn_args& a, int num_sms) {
   p.fd_gp = FastDiv(static_cast<uint32_t>(p.gp));
   const long long segs = static_cast<long long>(a.B) * p.tiles * p.groups;
   const int blocks = (a.Sk + kB - 1) / kB;
-  // Keys are cut where tiles do not fill the SMs (16 heads on 4, D 128, us cut /
-  // in row mode: 960 rows over 8,000 keys 107 / 122, 384 over 8,000 66 / 121,
-  // 64 rows of 8 heads on one over 30,000 85 / 416).
+  // A CTA per row tile, both pipelines on its blocks, where there is one tile a
+  // sequence or no more tiles than SMs; beyond that row mode, whose pipelines
+  // share each block (16 heads on 4, D 128, causal prompts of 152 / 200 / 296
+  // tiles: 29 / 35 / 47 us in row mode, 60 / 82 / 141 cut over the SMs; of 148
+  // tiles 44 in row mode, 41 with a CTA per tile).
   p.split = p.tiles == 1 || segs <= num_sms;
   if (p.split) {
-    // Short tiles stay whole and need no join: up to 4 blocks (one token over
-    // 500 keys, 16 sequences: 16.6 against 20.8 with cuts), up to 8 once there
-    // are tiles for a good part of the SMs (64 sequences of 900 keys 45 against
-    // 62, 800 rows of a prompt 23 against 47; but one sequence of 1,000 keys 22
-    // against 19).
-    p.whole = blocks <= 4 || (blocks <= 8 && segs >= 32);
+    // Tiles stay whole, without a join, while cutting them would not pay: the
+    // fewer SMs the tiles leave idle, the longer.  Steps of 16 heads on 4 at D
+    // 128, us cut / whole: 1 tile of 700 keys 21 / 21, of 1,300 21 / 28; 32
+    // tiles of 700 29 / 21, of 1,800 29 / 33; 64 of 1,800 36 / 33, of 4,000
+    // 52 / 62; 96 of 2,500 53 / 44, of 8,000 96 / 109; 148 of 4,000 80 / 66;
+    // prompts of 136 tiles over 5,000 keys 98 / 86, of 64 over 5,000 64 / 78.
+    // More tiles than SMs run in uneven waves when whole: 200 of 1,300 65 / 55,
+    // of 4,000 104 / 120.
+    const long long most_blocks = segs > num_sms ? 16 : 7 + 54 * segs * segs / (num_sms * num_sms);
+    p.whole = blocks <= most_blocks;
     // A CTA's least share: with 8 blocks instead of 4 one sequence of 2,000 keys
     // takes 26 us instead of 21, with 2 as long.
     p.unit_min = 4;
