@@ -227,3 +227,21 @@ def test_pieces_of_very_different_references(lead, near_end, dt):
         att(q, k, v, out=out)
         att.check()
         check_attention(out, out, attention_ref(q, k, v, 1.0))
+
+
+def test_an_object_that_dies_within_a_capture():
+    """Its handle is not freed there (that synchronizes, which a capture does not survive)."""
+    import yb_ops
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    q, k, v = (torch.randn(1, n, 2, 64, generator=g, device="cuda").bfloat16() for n in (1, 300, 300))
+    att, other = (yb_ops.Attention(2, 2, 64, torch.bfloat16) for _ in range(2))
+    want = att(q, k, v)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = att(q, k, v)
+        del other
+    graph.replay()
+    att.check()
+    assert torch.equal(out, want)

@@ -91,7 +91,8 @@ def _call(f, args, index: int) -> int:
 class Attention:
     """yb_attn_*: attention with optional score cap, distance bias, document and prefix masks.
 
-    One object serves any batch and length, on any stream; its handle lives on `device` (default: the current one)."""
+    One object serves any batch and length, on any stream; its handle lives on `device` (default: the current one).
+    Make it before a stream capture, and keep it while a graph that holds its calls is replayed."""
 
     def __init__(self, heads: int, kv_heads: int, head_dim: int, dtype, scale: float | None = None, cap: float = 0.0,
                  causal: bool = False, device=None):
@@ -122,19 +123,23 @@ class Attention:
 
     def __del__(self):
         try:
-            self.close()
+            # close() synchronizes, which would end a stream capture under way with an error; the few bytes stay.
+            if not torch.cuda.is_current_stream_capturing():
+                self.close()
         except Exception:
             pass
 
     def check(self) -> None:
-        """Synchronizes and raises if a kernel gave up a bounded wait."""
+        """Synchronizes and raises if a kernel gave up a bounded wait; rows of the calls since the last check may then
+        be wrong."""
         yb.check(yb.lib().yb_attn_check(self._h), "yb_attn_check")
 
     def __call__(self, q, k, v, out=None, q_len=None, k_len=None, prefix=None, key_range=None, slopes=None):
         """q [B, Sq, heads, D], k and v [B, Sk, kv_heads, D] -> out [B, Sq, heads, D].
 
         q_len, k_len, prefix int32 [B]; key_range int32 [B, Sq, 2]; slopes float32 [heads].  Rows past q_len keep
-        what `out` holds (zeros where it is allocated here)."""
+        what `out` holds (zeros where it is allocated here).  Does not synchronize: only check() tells of a kernel that
+        gave up a wait."""
         index, dt = self.device.index, self.dtype
         if q.dim() != 4 or k.dim() != 4:
             _fail("attention: q, k and v have four dimensions")
