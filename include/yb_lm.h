@@ -14,7 +14,8 @@
  * (which loads the kernels).  Strides are in elements and non-negative, given
  * as [batch, row, head]; the last dimension is contiguous.  Pointers lie on
  * their elements' boundaries (others are refused).  Lengths and positions are
- * read on the device, so that a captured graph follows them. */
+ * read on the device, so that a captured graph follows them.  No operator has
+ * a gradient. */
 
 #include <stddef.h>
 
@@ -37,11 +38,15 @@ typedef enum { YB_F32 = 0, YB_F16 = 1, YB_BF16 = 2 } yb_dtype;
  *         key_range[b][i][0] <= j < key_range[b][i][1]   when key_range
  *           (a document mask: the first key and the end of the row's document),
  *         j <= pos, or j < prefix[b] when prefix         when causal.
- * Key head h / (Hq / Hkv).  A row that sees no key gives zeros.  Rows i >=
- * q_len[b] of o keep their contents.  Keys that a row does not see do not
- * touch it, whatever they hold (infinities and NaN included).  A visible NaN
- * score, or one of +infinity, makes the row NaN.  Scores, sums and o are formed
- * in fp32; the weights enter the second product rounded to dtype. */
+ * Key head h / (Hq / Hkv).  A row that sees no key gives zeros, as does one
+ * whose visible scores are all -infinity.  Rows i >= q_len[b] of o keep their
+ * contents.  Keys that a row does not see do not touch it, whatever they hold
+ * (infinities and NaN included; a row that shares a block with such values is
+ * computed twice, slowly).  A visible s_j of NaN or +infinity makes the row NaN.
+ * Scores, sums and o are formed in fp32.  A capped score is within 16 2^-24 of
+ * its value (a cap above 2^20 times the scale: up to 4e-4 of the cap, and within
+ * 2^-22 of the cap beyond).  The weights enter the second product rounded to
+ * dtype. */
 typedef struct {
     const void* q; /* [B, Sq, Hq, D]  */
     const void* k; /* [B, Sk, Hkv, D] */
@@ -61,7 +66,8 @@ typedef struct {
 } yb_attn_args;
 
 /* A handle holds the error word of the kernels' bounded waits; it may be used
- * from any number of streams at once. */
+ * from any number of streams at once.  Create it outside stream captures, and
+ * keep it while a graph that holds its runs is replayed. */
 status_t yb_attn_create(int device, void** attn);
 
 /* Scratch bytes that yb_attn_run needs for these sizes (may be 0).  Calls that
@@ -75,7 +81,9 @@ status_t yb_attn_workspace(void* attn, const yb_attn_args* a, size_t* bytes);
  * 16-byte aligned, at least yb_attn_workspace bytes. */
 status_t yb_attn_run(void* attn, const yb_attn_args* a, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Synchronizes the device, reads and clears the error word. */
+/* Synchronizes the device, reads and clears the error word.  ERROR_DEVICE: a
+ * kernel gave up a wait (2 s, and 32 us a key, a minute at most) since the last
+ * check, and rows of its output are wrong; nothing else tells. */
 status_t yb_attn_check(void* attn);
 status_t yb_attn_destroy(void* attn);
 
@@ -91,7 +99,8 @@ status_t yb_attn_debug_withhold(void* attn);
  * then pair i of the first R dimensions is rotated by the angle
  * positions[b][t] * inv_freq[i] (radians; formed and reduced to one turn in 64
  * bits): pairs (i, i + R/2), or (2i, 2i + 1) when interleaved.  fp32 between
- * the load and the store (a sum of squares past its range gives zeros).
+ * the load and the store (a sum of squares above its range gives zeros; with
+ * eps = 0 one that vanishes gives infinities or NaN).
  * q -> q_out[b][t]; k -> k_out[b][start[b] + t], and v, unchanged, to the same
  * row of v_out: rows of a cache.  Rows outside [0, cache_rows) are not
  * written; nothing else of the outputs is touched.  q_out may be q, and, when
@@ -127,13 +136,13 @@ status_t yb_qk_norm_rope(const yb_qk_args* a, void* stream);
  *   top_k > 0: the first top_k of them;
  *   top_p < 1: of these, each whose forerunners hold less than top_p of their
  *              whole weight (the first one always);
- *   min_p > 0: of these, each with w_i >= min_p (the first one always);
+ *   min_p > 0: of these, each with w_i >= min_p (above 1 it counts as 1);
  * token[b] is the first of the kept ones, by rising index, whose running sum
  * of weights exceeds u[b] times their whole weight, and logprob[b] the log of
- * its share of that weight.  temperature <= 0 or NaN: the largest logit, with
- * logprob 0.  Logits of -infinity or NaN are never chosen, +infinity counts
- * as the largest finite float; a row without any other logit gives token -1
- * and logprob -infinity.  u is clamped to [0, 1).  Weights are held as whole
+ * its share of that weight (from its logit, in 64 bits).  temperature <= 0 or
+ * NaN: the largest logit, with logprob 0.  Logits of -infinity or NaN are never
+ * chosen, +infinity counts as the largest finite float; a row without any other
+ * logit gives token -1 and logprob -infinity.  u is clamped to [0, 1).  Weights are held as whole
  * numbers of 2^-44, so that sums do not depend on their order; a token below
  * 2^-45 of the largest weight is never chosen. */
 typedef struct {

@@ -41,16 +41,20 @@
 //
 // Rounding: P is rounded to the operands' type (they enter the same UMMA); its
 // sum is taken before that in fp32.  O, maxima and sums are fp32 throughout.
+// Against 64 bits the error is up to 1.4 times that of fp32 weights rounded once
+// at the end (2 x 4,096 capped rows 0.0022 against 0.0016, one fp16 token over
+// 401 keys 0.00028 against 0.00021).
 //
 // What bounds it.  D = 128: a block pair (256 rows, 128 keys) takes 2,048 clocks
 // of tensor work (4,096 multiply-adds a clock) and 2,048 of exponentials (16 a
 // clock), which overlap in part, and the scores of 64 keys, whose Q is read
 // from shared memory again for each half, take 384 clocks instead of 256: 2 x
-// 4,096 capped causal rows of 16 heads 157 us, 0.87 PFLOP/s.  D = 64: the
+// 4,096 capped causal rows of 16 heads 154 to 178 us (0.89 to 0.77 PFLOP/s; the
+// longer the more work runs around them).  D = 64: the
 // exponentials (about 10 clocks a warp's 32 instead of 8 in practice).  Short
 // tiles (documents, a few blocks each): 2 us of start-up and 2 us of output a
 // CTA, which nothing overlaps with one CTA per SM.  Split mode: 24 sequences of
-// up to 16,384 keys 210 us, 3.98 TB/s, 0.61 of the measured copy rate; the UMMA
+// up to 16,384 keys 198 us, 4.2 TB/s, 0.64 of the measured copy rate; the UMMA
 // warp's waits and products of 128 rows (4 of them in use) stand between ring
 // and memory.
 #include <cuda.h>

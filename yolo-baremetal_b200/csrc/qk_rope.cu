@@ -11,7 +11,7 @@
 // Norm and rotation are fp32 on pairs, rounded once on the way out.
 //
 // The bound is DRAM (each row read and written once): 8,191 tokens of 48 bf16
-// head rows of 128 take 53.6 us, 3.75 TB/s, 0.57 of the measured copy rate.
+// head rows of 128 take 53.5 to 54.5 us, 3.7 TB/s, 0.57 of the measured copy rate.
 // What is in the way is instructions, two thirds of the issue slots before
 // addresses moved into a per-token table, the weights into shared memory and
 // the arithmetic onto pairs (62 us then).
@@ -278,8 +278,8 @@ cudaError_t launch(const yb_qk_args& a, cudaStream_t s) {
   while (group_log < 5 && (1 << group_log) < slots) ++group_log;
   const long long total = static_cast<long long>(a.B) * a.S;
   // A token per CTA spreads a decode step over the SMs; four share what comes
-  // before their rows once there are CTAs enough for two on each SM (3,003
-  // fp32 tokens: 20.6 us one by one, 14.4 by fours).
+  // before their rows once there are CTAs enough for two on each of 148 SMs
+  // (3,003 fp32 tokens: 20.6 us one by one, 14.4 by fours).
   const int tokens = total >= 2 * 148 * kMaxTokens ? kMaxTokens : 1;
   const unsigned grid = static_cast<unsigned>((total + tokens - 1) / tokens);
   if (a.interleaved)

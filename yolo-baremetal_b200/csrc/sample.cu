@@ -26,7 +26,7 @@
 // Measured: one row of 32,000 fp32 logits with top-k 50 and top-p 0.95 10.8 us
 // in the kernel, of which the cluster's four barriers and the exchange of the
 // histogram are about half: latency.  256 unfiltered rows of 131,072 fp32
-// logits 87 us (1.5 TB/s): about 45 instructions and 14 fp64 operations a
+// logits 87 us (1.5 TB/s): about 50 instructions and 14 fp64 operations a
 // token, half of the issue slots; the rest are the barriers between the load,
 // the maximum and the sums, with three CTAs an SM to fill them.
 #include <cooperative_groups.h>
@@ -105,7 +105,7 @@ struct Row {
 // 2^y = 2^n 2^(j/64) 2^r with |r| <= 1/128 (table-driven, after Tang 1989): the
 // Taylor polynomial of degree 4 leaves (r ln 2)^5 / 120 < 2^-44.  Rounding to
 // whole numbers is done by adding 1.5 2^52 and 2^52: twelve fp64 operations and
-// one conversion (they run at a quarter of the fp64 rate).
+// one conversion (they run at a quarter of the fp64 rate), fourteen with the sum.
 __device__ __forceinline__ double weight_d(float x, const Row& r, const double* table) {
   const double y = (static_cast<double>(x) - r.best) * r.c;
   const double t = fma(y, 64.0, 6755399441055744.0);
@@ -260,7 +260,6 @@ struct Picker {
         o->tcnt[me * share + i] = c;
         if (with_mass) o->tmass[me * share + i] = m;
       }
-      if (share > kThreads && i + kThreads >= share) break;
     }
     cl.sync();
     // Running sums.
@@ -628,7 +627,7 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
   }
 
   // Kept weights of each warp's run, as whole fp64 numbers (at most 2^44 times
-  // 64 tokens a lane: exact).
+  // 65 tokens a lane: exact).
   const float edge = cut ? value_of(cut) : -INFINITY;
   const double least = static_cast<double>(s.least);
   auto kept = [&](int j) -> double {  // of raw[j]
@@ -688,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, FILTER ? 2 : 3) sample_kernel(const 
 template <typename T, bool FILTER>
 status_t launch_sample(const yb_sample_args& a, cudaStream_t s) {
   // Slices of at most 16384 tokens; smaller ones while the CTAs do not fill
-  // the SMs twice and each thread still has four tokens.
+  // the 148 SMs twice and each thread still has four tokens.
   int C = 1;
   while (C < kMaxCluster && ((a.V + C - 1) / C > 16384 ||
                              (static_cast<long long>(a.B) * C < 2 * 148 && (a.V + C - 1) / C > 4 * kThreads)))
