@@ -44,9 +44,9 @@ typedef enum { YB_F32 = 0, YB_F16 = 1, YB_BF16 = 2 } yb_dtype;
  * (infinities and NaN included; a row that shares a block with such values is
  * computed twice, slowly).  A visible s_j of NaN or +infinity makes the row NaN.
  * Scores, sums and o are formed in fp32.  A capped score is within 16 2^-24 of
- * its value (a cap above 2^20 times the scale: up to 4e-4 of the cap, and within
- * 2^-22 of the cap beyond).  The weights enter the second product rounded to
- * dtype. */
+ * its value, or within 2^-22 of the cap where that is more than 2^20 times below
+ * the scale, or more than 2^20 times above it and the score past 4e-4 of it.  The
+ * weights enter the second product rounded to dtype. */
 typedef struct {
     const void* q; /* [B, Sq, Hq, D]  */
     const void* k; /* [B, Sk, Hkv, D] */
